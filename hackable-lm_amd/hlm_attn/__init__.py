@@ -12,9 +12,13 @@ Public surface:
   LMHeadProjection                            model.py's LM head with fwd_hip
   residual_rms_norm_hip                       residual add + RMSNorm (OutputProjection / DownProjection)
   OutputProjection, DownProjection            model.py's projections with fwd_hip
+  KVCache                                     one layer's 8-bit key/value cache
+  kv_cache_write_hip, kv_cache_read_hip       storing tokens in it, reading them back
+  cached_attention_hip                        attention of new tokens over it, with an optional prefix shared by the batch
 The kernels live in libhlm_attn.so (built by hlm_attn.build), reached through
 the C ABI in include/hlm_attn.h.
 """
+from .cache import KVCache
 from .config import (
     ATTENTION_BACKENDS,
     HIP_BACKEND,
@@ -28,8 +32,11 @@ from .config import (
 )
 from .kernels import (
     attention,
+    cached_attention_hip,
     fused_linear_cross_entropy_with_weight,
     hip_attention_available,
+    kv_cache_read_hip,
+    kv_cache_write_hip,
     qk_norm_rope_hip,
     residual_rms_norm_hip,
     resolve_attention_backend,
@@ -65,6 +72,10 @@ __all__ = [
     "RotaryEmbedding",
     "qk_norm_rope_hip",
     "residual_rms_norm_hip",
+    "KVCache",
+    "cached_attention_hip",
+    "kv_cache_read_hip",
+    "kv_cache_write_hip",
     "OutputProjection",
     "DownProjection",
     "resolve_attention_backend",

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "attn_common.h"
+#include "kv_cache.h"
 #include "../../../include/hlm_attn.h"
 
 namespace hlm {
@@ -31,6 +32,12 @@ hipError_t launch_lm_head_dhidden(const void* g, int64_t ldg, const void* w, int
                                   int M, int N, int K, hipStream_t stream);
 hipError_t launch_residual_rms_norm(const void* a, const void* b, const void* c, void* y0, void* y1, int64_t rows,
                                     int n, float eps, bool backward, hipStream_t stream);
+template <int D>
+hipError_t launch_cache_io(const CacheIoArgs& p, bool write, hipStream_t stream);
+template <int D>
+int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys);
+template <int D>
+hipError_t launch_cached_attn(CachedAttnArgs& p, hipStream_t stream);
 }  // namespace hlm
 
 namespace {
@@ -602,6 +609,178 @@ int hlm_residual_rms_norm_fwd(const void* residual, const void* branch, void* ou
 int hlm_residual_rms_norm_bwd(const void* out, const void* grad_out, const void* grad_normed, void* grad_in,
                               int64_t rows, int n, float eps, void* stream) {
   return run_residual_rms_norm(true, out, grad_out, grad_normed, grad_in, nullptr, rows, n, eps, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+constexpr int kMaxSlots = 1 << 24;  // a head's bytes, slots x 128, stay below 2^31
+
+// Strides of dims of one index are not looked at.
+int check_rows(const char* name, const void* p, const int64_t* s, int B, int T, int heads) {
+  if (p == nullptr || !aligned16(p)) return fail(HLM_ATTN_EINVAL, "%s is null or not 16-byte aligned", name);
+  if (s == nullptr) return fail(HLM_ATTN_EINVAL, "%s strides are a null pointer", name);
+  const int n[3] = {B, T, heads};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] < 0 || s[i] % 8 != 0))
+      return fail(HLM_ATTN_EINVAL, "%s stride[%d] = %lld must be a non-negative multiple of 8 elements", name, i,
+                  (long long)s[i]);
+  return HLM_ATTN_OK;
+}
+
+int check_cache(const char* name, const void* k, const void* v, const float* ks, const float* vs, int slots) {
+  if (slots <= 0 || slots % hlm::kCacheBlock != 0 || slots > kMaxSlots)
+    return fail(HLM_ATTN_EINVAL, "%s slots %d must be a multiple of %d in [%d, %d]", name, slots, hlm::kCacheBlock,
+                hlm::kCacheBlock, kMaxSlots);
+  for (const void* p : {k, v, static_cast<const void*>(ks), static_cast<const void*>(vs)})
+    if (p == nullptr || !aligned16(p)) return fail(HLM_ATTN_EINVAL, "a %s tensor is null or not 16-byte aligned", name);
+  return HLM_ATTN_OK;
+}
+
+// Places that the host knows have to lie inside the cache.
+int check_span(const int* starts, int start, const int* counts, int T, int slots) {
+  if (starts == nullptr && (start < 0 || start > slots || (counts == nullptr && (int64_t)start + T > slots)))
+    return fail(HLM_ATTN_EINVAL, "%d tokens at position %d do not fit a cache of %d", T, start, slots);
+  return HLM_ATTN_OK;
+}
+
+int run_cache_io(bool write, const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides, void* k_out,
+                 void* v_out, void* cache_k, void* cache_v, float* k_scale, float* v_scale, int slots, const int* starts,
+                 int start, const int* counts, int B, int T, int Hkv, int D, void* stream) {
+  g_last_error[0] = '\0';
+  if (B < 0 || T < 0 || Hkv <= 0) return fail(HLM_ATTN_EINVAL, "bad shape B=%d T=%d Hkv=%d", B, T, Hkv);
+  if (D != 64 && D != 128) return fail(HLM_ATTN_EUNSUPPORTED, "head_dim %d is not supported (64 or 128)", D);
+  if ((int64_t)B * T >= ((int64_t)1 << 31) || (int64_t)B * T * Hkv >= ((int64_t)1 << 34))
+    return fail(HLM_ATTN_EUNSUPPORTED, "too many rows for one launch");
+  int rc = check_span(starts, start, counts, T, slots);
+  if (rc) return rc;
+  if (B == 0 || T == 0) return HLM_ATTN_OK;
+  if ((rc = check_cache("cache", cache_k, cache_v, k_scale, v_scale, slots))) return rc;
+  if (write && ((rc = check_rows("k", k, k_strides, B, T, Hkv)) || (rc = check_rows("v", v, v_strides, B, T, Hkv))))
+    return rc;
+  if (!write && (k_out == nullptr || v_out == nullptr || !aligned16(k_out) || !aligned16(v_out)))
+    return fail(HLM_ATTN_EINVAL, "an output is null or not 16-byte aligned");
+  hlm::CacheIoArgs a{};
+  a.cache = {static_cast<uint8_t*>(cache_k), static_cast<uint8_t*>(cache_v), k_scale, v_scale, slots};
+  a.span = {starts, counts, start, T};
+  a.k = static_cast<const hlm::bf16*>(k);
+  a.v = static_cast<const hlm::bf16*>(v);
+  if (write) {
+    copy3(a.sk, k_strides);
+    copy3(a.sv, v_strides);
+  }
+  a.k_out = static_cast<hlm::bf16*>(k_out);
+  a.v_out = static_cast<hlm::bf16*>(v_out);
+  a.B = B;
+  a.Hkv = Hkv;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t err = D == 64 ? hlm::launch_cache_io<64>(a, write, s) : hlm::launch_cache_io<128>(a, write, s);
+  if (err != hipSuccess) return fail(HLM_ATTN_ELAUNCH, "cache launch failed: %s", hipGetErrorString(err));
+  return HLM_ATTN_OK;
+}
+
+// The sizes of a cached attention and its plan.
+int plan_cached(hlm::CachedAttnArgs& a, int64_t& ws_floats, int B, int T, int H, int Hkv, int D, int slots,
+                const int* starts, int start, const int* counts, int prefix_length, int window) {
+  if (B < 0 || T < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0)
+    return fail(HLM_ATTN_EINVAL, "bad shape B=%d T=%d H=%d Hkv=%d", B, T, H, Hkv);
+  if (D != 64 && D != 128) return fail(HLM_ATTN_EUNSUPPORTED, "head_dim %d is not supported (64 or 128)", D);
+  if (slots <= 0 || slots % hlm::kCacheBlock != 0 || slots > kMaxSlots)
+    return fail(HLM_ATTN_EINVAL, "cache slots %d must be a multiple of %d in [%d, %d]", slots, hlm::kCacheBlock,
+                hlm::kCacheBlock, kMaxSlots);
+  if (prefix_length < 0 || prefix_length > kMaxSlots) return fail(HLM_ATTN_EINVAL, "bad prefix length %d", prefix_length);
+  if (const int rc = check_span(starts, start, counts, T, slots)) return rc;
+  // rows are counted, and the partial sums' rows addressed, in ints
+  if ((int64_t)B * T > ((int64_t)1 << 30) || (int64_t)B * T * H > ((int64_t)1 << 30))
+    return fail(HLM_ATTN_EUNSUPPORTED, "too many query rows for one launch");
+  ws_floats = 0;
+  a.span = {starts, counts, start, T};
+  a.B = B;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.G = H / Hkv;
+  a.P = prefix_length;
+  a.window = window > 0 ? window : 0x7fffffff;
+  if (B == 0 || T == 0) return HLM_ATTN_OK;
+  const int64_t keys = starts == nullptr ? std::min<int64_t>(slots, (int64_t)start + T) : slots;
+  const int64_t items = D == 64 ? hlm::plan_cached_attn<64>(a, keys) : hlm::plan_cached_attn<128>(a, keys);
+  if (items >= ((int64_t)1 << 31)) return fail(HLM_ATTN_EUNSUPPORTED, "problem too large for one launch");
+  const int splits = a.own_splits + a.prefix_splits;
+  ws_floats = splits == 1 ? 0 : (int64_t)splits * B * T * H * (D + 2);
+  return HLM_ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hlm_attn_cache_write(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides, void* cache_k,
+                         void* cache_v, float* k_scale, float* v_scale, int slots, const int32_t* starts, int start,
+                         const int32_t* counts, int B, int T, int Hkv, int D, void* stream) {
+  return run_cache_io(true, k, v, k_strides, v_strides, nullptr, nullptr, cache_k, cache_v, k_scale, v_scale, slots, starts,
+                      start, counts, B, T, Hkv, D, stream);
+}
+
+int hlm_attn_cache_read(const void* cache_k, const void* cache_v, const float* k_scale, const float* v_scale, int slots,
+                        void* k, void* v, const int32_t* starts, int start, const int32_t* counts, int B, int T, int Hkv,
+                        int D, void* stream) {
+  return run_cache_io(false, nullptr, nullptr, nullptr, nullptr, k, v, const_cast<void*>(cache_k), const_cast<void*>(cache_v),
+                      const_cast<float*>(k_scale), const_cast<float*>(v_scale), slots, starts, start, counts, B, T, Hkv, D,
+                      stream);
+}
+
+int64_t hlm_attn_cached_fwd_workspace_bytes(int B, int T, int H, int Hkv, int D, int slots, const int32_t* starts, int start,
+                                            const int32_t* counts, int prefix_length, int window) {
+  g_last_error[0] = '\0';
+  hlm::CachedAttnArgs a{};
+  int64_t floats = 0;
+  if (const int rc = plan_cached(a, floats, B, T, H, Hkv, D, slots, starts, start, counts, prefix_length, window)) return rc;
+  return floats * 4;
+}
+
+int hlm_attn_cached_fwd(const void* q, const int64_t* q_strides, void* o, const void* cache_k, const void* cache_v,
+                        const float* k_scale, const float* v_scale, int slots, const int32_t* starts, int start,
+                        const int32_t* counts, const void* prefix_k, const void* prefix_v, const float* prefix_k_scale,
+                        const float* prefix_v_scale, int prefix_slots, int prefix_length, int B, int T, int H, int Hkv,
+                        int D, int window, float scale, void* ws, int64_t ws_bytes, void* stream) {
+  g_last_error[0] = '\0';
+  hlm::CachedAttnArgs a{};
+  int64_t floats = 0;
+  int rc = plan_cached(a, floats, B, T, H, Hkv, D, slots, starts, start, counts, prefix_length, window);
+  if (rc) return rc;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(HLM_ATTN_EINVAL, "scale must be positive and finite");
+  if (B == 0 || T == 0) return HLM_ATTN_OK;
+  if ((rc = check_rows("q", q, q_strides, B, T, H)) || (rc = check_cache("cache", cache_k, cache_v, k_scale, v_scale, slots)))
+    return rc;
+  if (o == nullptr || !aligned16(o)) return fail(HLM_ATTN_EINVAL, "o is null or not 16-byte aligned");
+  if (prefix_length > 0) {
+    if ((rc = check_cache("prefix", prefix_k, prefix_v, prefix_k_scale, prefix_v_scale, prefix_slots))) return rc;
+    if (prefix_length > prefix_slots)
+      return fail(HLM_ATTN_EINVAL, "prefix length %d is beyond its %d slots", prefix_length, prefix_slots);
+  }
+  if (floats > 0 && (ws == nullptr || !aligned16(ws)))
+    return fail(HLM_ATTN_EINVAL, "workspace is null or not 16-byte aligned");
+  if (ws_bytes < floats * 4)
+    return fail(HLM_ATTN_EINVAL, "workspace holds %lld bytes, %lld needed", (long long)ws_bytes, (long long)floats * 4);
+  const auto cache = [](const void* k, const void* v, const float* ks, const float* vs, int n) {
+    return hlm::KvCache{static_cast<uint8_t*>(const_cast<void*>(k)), static_cast<uint8_t*>(const_cast<void*>(v)),
+                        const_cast<float*>(ks), const_cast<float*>(vs), n};
+  };
+  a.q = static_cast<const hlm::bf16*>(q);
+  copy3(a.sq, q_strides);
+  a.o = static_cast<hlm::bf16*>(o);
+  a.own = cache(cache_k, cache_v, k_scale, v_scale, slots);
+  a.prefix = cache(prefix_k, prefix_v, prefix_k_scale, prefix_v_scale, prefix_slots);
+  a.scale_log2 = scale * hlm::kLog2e;
+  a.div_G = hlm::fast_div_of((unsigned)a.G);
+  a.div_T = hlm::fast_div_of((unsigned)T);
+  a.part_o = static_cast<float*>(ws);
+  a.part_ml = a.part_o + floats / (D + 2) * D;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipError_t err = D == 64 ? hlm::launch_cached_attn<64>(a, s) : hlm::launch_cached_attn<128>(a, s);
+  if (err != hipSuccess) return fail(HLM_ATTN_ELAUNCH, "cached attention launch failed: %s", hipGetErrorString(err));
+  return HLM_ATTN_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,90 @@
+// The 8-bit key/value cache and the arguments of the kernels over it.
+//
+// One layer's cache of B sequences, Hkv heads of D values and S slots (token
+// positions, a multiple of 64).  A row x (one token's key or value of one kv
+// head) is held as whole numbers c = -127 .. 127, stored as the bytes c + 128,
+// and one fp32 scale:
+//     a = max |x_d|,   scale = a / 127,   c_d = 127 x_d / a  (nearest, ties to even),
+// so x_d ~ c_d scale with an error of at most half a scale.  A row whose a is
+// below 2^-119 is held as zeros (its scale would leave the normal fp32 range);
+// one that holds an infinity or a NaN gets the scale NaN and reads as NaN.
+//
+//   keys    k  bytes (B, Hkv, S, D)
+//   values  v  bytes (B, Hkv, S / 64, D, 64): blocks of 64 tokens, transposed
+//   k_scale, v_scale  fp32 (B, Hkv, S)
+//
+// Keys and values of one head are contiguous, 64 D bytes to a 64-token block.
+// The values' blocks are transposed because the products contract q.k over D
+// and p.v over tokens: both of their matrix operands then come out of memory
+// as 16 contiguous bytes of a lane, without a pass through LDS.
+//
+// Token t of sequence b lies at position starts[b] + t (`start` for all
+// sequences where starts is null).  Tokens t >= counts[b], and positions
+// outside 0 .. S - 1, are padding: they are not written, read as zeros, and
+// their queries' output rows are zeros.
+#pragma once
+
+#include "attn_common.h"
+
+namespace hlm {
+
+constexpr int kCacheBlock = 64;  // tokens of a block
+constexpr float kCacheTiny = 1.504632769052528e-36f;  // 2^-119
+
+struct KvCache {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int slots;
+};
+
+// The new tokens' places.
+struct CacheSpan {
+  const int* starts;
+  const int* counts;  // null: T each
+  int start;
+  int T;
+};
+
+// The position of token t of sequence b, or -1 for padding.
+__device__ __forceinline__ int64_t span_start(const CacheSpan& s, int b) { return s.starts ? s.starts[b] : s.start; }
+__device__ __forceinline__ int span_count(const CacheSpan& s, int b) {
+  return s.counts ? min(s.counts[b], s.T) : s.T;
+}
+__device__ __forceinline__ int cache_position(int64_t start, int count, int t, int slots) {
+  const int64_t p = start + t;
+  return t < count && p >= 0 && p < slots ? (int)p : -1;
+}
+
+struct CacheIoArgs {
+  KvCache cache;
+  CacheSpan span;
+  const bf16* k;  // write: inputs (B, T, Hkv, D), unit D stride
+  const bf16* v;
+  int64_t sk[3], sv[3];
+  bf16* k_out;  // read: outputs (B, T, Hkv, D), contiguous
+  bf16* v_out;
+  int B, Hkv;
+  int blocks;  // 64-token blocks that T tokens can touch
+};
+
+struct CachedAttnArgs {
+  const bf16* q;
+  int64_t sq[3];
+  bf16* o;  // (B, T, H, D), contiguous
+  KvCache own, prefix;  // prefix of one sequence; prefix.slots 0: none
+  CacheSpan span;
+  int B, H, Hkv, G;
+  int P;       // prefix tokens
+  int window;  // >= 1
+  float scale_log2;
+  FastDiv div_G, div_T;
+  // Splits of the keys: own_splits workgroups share a sequence's keys (for one
+  // tile of its rows), prefix_splits the prefix's.
+  int own_splits, prefix_splits, own_tiles, prefix_tiles, prefix_items;
+  float* part_o;   // (splits, B T H, D), unnormalised
+  float* part_ml;  // (splits, B T H, 2): running maximum in log2 units and sum
+};
+
+}  // namespace hlm

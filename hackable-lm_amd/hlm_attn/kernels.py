@@ -25,12 +25,15 @@ kernels.py:945-959: the HIP cross-entropy rows in place of the Triton
 from __future__ import annotations
 
 import math
-from typing import Any
+from typing import TYPE_CHECKING, Any
 
 import torch
 
 from . import _lib
 from .config import HIP_BACKEND, normalize_attention_backend
+
+if TYPE_CHECKING:
+    from .cache import KVCache
 
 
 def hip_attention_available() -> bool:
@@ -335,3 +338,107 @@ def residual_rms_norm_hip(residual: torch.Tensor, branch: torch.Tensor, eps: flo
     if out is not None:
         return out
     return ops.hip_residual_rms_norm(residual, branch, float(eps))
+
+
+# --- generation and scoring over an 8-bit key/value cache --------------------------
+#
+# No counterpart in the reference, whose adapter runs the whole sequence again
+# for each new token (lm_eval_hackable_lm.py:185-207).
+
+
+def _places(starts: torch.Tensor | int) -> tuple[torch.Tensor | None, int]:
+    return (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+
+
+def _head_padded(x: torch.Tensor, cache: "KVCache", name: str) -> torch.Tensor:
+    """x as bf16 with the cache's kernel head dim, zero-padded where head_dim is none."""
+    if x.dim() != 4 or x.shape[-1] != cache.head_dim:
+        raise RuntimeError(f"{name} {tuple(x.shape)} does not have 4 dims with heads of {cache.head_dim}")
+    if x.dtype is not torch.bfloat16:
+        x = x.to(torch.bfloat16)
+    pad = cache.kernel_dim - cache.head_dim
+    return torch.nn.functional.pad(x, (0, pad)) if pad else x
+
+
+def kv_cache_write_hip(
+    cache: "KVCache", k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor | int, counts: torch.Tensor | None = None
+) -> None:
+    """Stores k and v (B, T, Hkv, D) in `cache`: token t of sequence b at
+    position starts[b] + t.
+
+    starts: the first position, one int for all sequences or a device tensor
+    (B,) of int32 (int64 is converted).  counts: how many of the T tokens of
+    each sequence are real, the first ones (None: all); the others, and those
+    at positions outside the cache, are not written.  An int that does not fit
+    the cache raises; a tensor's values are never read by the host, so the call
+    can be captured and replayed.  Each row is held as whole numbers -127 .. 127
+    relative to its largest value, an error of at most 1/254 of it.  Values
+    other than bf16 are rounded to it first.  No backward: tensors that require
+    grad are refused outside torch.no_grad()."""
+    ops = _ops or _load_ops()
+    if k.shape[-1] != cache.head_dim or v.shape != k.shape:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache with heads of {cache.head_dim}")
+    k, v = _head_padded(k, cache, "k"), _head_padded(v, cache, "v")
+    run = ops.kv_cache_write_impl if ops.direct_call_ok(k, v) else ops.hip_kv_cache_write
+    run(k, v, *cache.tensors(), *_places(starts), counts)
+
+
+def kv_cache_read_hip(
+    cache: "KVCache", starts: torch.Tensor | int, length: int, counts: torch.Tensor | None = None
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values of `length` tokens from starts on, as bf16
+    (B, length, Hkv, D); starts and counts as in kv_cache_write_hip.  Padding
+    and positions outside the cache, or never written, are zeros."""
+    ops = _ops or _load_ops()
+    run = ops.kv_cache_read_impl if ops.direct_call_ok(cache.k) else ops.hip_kv_cache_read
+    k, v = run(*cache.tensors(), *_places(starts), counts, int(length))
+    return (k, v) if cache.kernel_dim == cache.head_dim else (k[..., : cache.head_dim], v[..., : cache.head_dim])
+
+
+def cached_attention_hip(
+    q: torch.Tensor,
+    cache: "KVCache",
+    starts: torch.Tensor | int,
+    counts: torch.Tensor | None = None,
+    window_size: int | None = None,
+    scale: float | None = None,
+    prefix: "KVCache | None" = None,
+    prefix_length: int = 0,
+) -> torch.Tensor:
+    """Causal (sliding-window) attention of T new tokens per sequence over a
+    cache: q (B, T, H, D) -> bf16 (B, T, H, D), H a multiple of the cache's kv
+    heads.
+
+    Query t of sequence b stands at position p = starts[b] + t and sees the
+    cached positions max(0, p - W + 1) .. p (W = window_size; None: all), so
+    kv_cache_write_hip has stored its own key and value before.  T is 1 for
+    generation, a few for drafted tokens, more for a chunk of a prompt; starts
+    and counts are as in kv_cache_write_hip, and rows of padding come out as
+    zeros.
+
+    prefix: a cache of one sequence whose first prefix_length tokens stand
+    before every sequence's own (at positions 0 .. prefix_length - 1, the own
+    ones behind them): its keys and values are read once for the whole batch.
+    starts still counts own tokens, and the window reaches back into the prefix.
+
+    No backward: q that requires grad is refused outside torch.no_grad()."""
+    ops = _ops or _load_ops()
+    if window_size is not None and window_size < 1:
+        raise RuntimeError(f"window_size must be >= 1 or None, got {window_size}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(cache.head_dim)
+    if prefix is None:
+        shared: tuple = (None, None, None, None)
+        if prefix_length:
+            raise RuntimeError(f"prefix_length {prefix_length} without a prefix")
+    else:
+        if prefix.head_dim != cache.head_dim:
+            raise RuntimeError(f"prefix heads of {prefix.head_dim} and cache heads of {cache.head_dim} differ")
+        if not 0 <= prefix_length <= prefix.capacity:
+            raise RuntimeError(f"prefix_length {prefix_length} is outside 0 .. {prefix.capacity}")
+        shared = prefix.tensors()
+    q = _head_padded(q, cache, "q")
+    run = ops.cached_attn_impl if ops.direct_call_ok(q) else ops.hip_cached_attn
+    out = run(q, *cache.tensors(), *_places(starts), counts, *shared, int(prefix_length),
+              0 if window_size is None else int(window_size), float(scale))
+    return out if cache.kernel_dim == cache.head_dim else out[..., : cache.head_dim]

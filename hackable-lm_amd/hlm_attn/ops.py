@@ -690,3 +690,187 @@ def _res_backward(ctx, grad_out, grad_normed):
 
 
 hip_residual_rms_norm.register_autograd(_res_backward, setup_context=_res_setup_context)
+
+
+# --- the 8-bit key/value cache and attention over it ------------------------------
+#
+# hackable_lm::hip_kv_cache_write (mutates the cache), hip_kv_cache_read and
+# hip_cached_attn.  No backward: they serve generation and scoring.  Places are
+# an int (all sequences) or an int32 / int64 device tensor of one per sequence.
+
+
+def _no_grad_only(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"hip {what} has no backward: call it under torch.no_grad()")
+
+
+def _per_sequence(name: str, x: torch.Tensor | None, batch: int, device: torch.device) -> torch.Tensor | None:
+    """starts or counts as the kernels read them: int32 (batch,), contiguous."""
+    if x is None:
+        return None
+    if x.device != device or x.shape != (batch,) or x.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name} must be int32 or int64 of shape ({batch},) on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if x.dtype is not torch.int32:  # positions beyond int32 are outside of every cache, and stay so
+        x = x.clamp(-(2**31), 2**31 - 1).to(torch.int32)
+    return x.contiguous()
+
+
+def _check_cache_tensors(name: str, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    B, Hkv, S, D = k.shape
+    if (k.dtype is not torch.uint8 or v.dtype is not torch.uint8 or k_scale.dtype is not torch.float32
+            or v_scale.dtype is not torch.float32 or v.shape != (B, Hkv, S // 64, D, 64) or k_scale.shape != (B, Hkv, S)
+            or v_scale.shape != (B, Hkv, S)):
+        raise RuntimeError(f"the {name} tensors are not those of a KVCache")
+    for t in (k, v, k_scale, v_scale):
+        if t.device != k.device or not t.is_contiguous():
+            raise RuntimeError(f"the {name} tensors must be contiguous and on one device")
+
+
+def _row_strides(t: torch.Tensor) -> ctypes.Array:
+    """strides3 for the cache's entry points, which look at no stride of a dim of one index."""
+    return _lib.strides3(t)
+
+
+def _cache_rows(name: str, t: torch.Tensor, cache_k: torch.Tensor) -> torch.Tensor:
+    """New rows (B, T, heads, D) in a layout that the cache kernels read in place, or a copy."""
+    if t.device.type != "cuda":
+        raise RuntimeError(f"hip kv cache runs on ROCm devices only, got {name} on {t.device}")
+    if t.dtype is not _BF16 or t.dim() != 4:
+        raise RuntimeError(f"hip kv cache expects bfloat16 {name} shaped (B, T, heads, D), got {t.dtype} {tuple(t.shape)}")
+    if t.device != cache_k.device or t.shape[0] != cache_k.shape[0] or t.shape[3] != cache_k.shape[3]:
+        raise RuntimeError(f"{name} {tuple(t.shape)} on {t.device} does not match a cache of {tuple(cache_k.shape)} on {cache_k.device}")
+    s = t.stride()
+    fits = s[3] == 1 and not t.data_ptr() & 15 and all(n <= 1 or (x >= 0 and not x & 7) for n, x in zip(t.shape[:3], s))
+    return t if fits else t.contiguous()
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def kv_cache_write_impl(
+    k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor,
+    v_scale: torch.Tensor, starts: torch.Tensor | None, start: int, counts: torch.Tensor | None,
+) -> None:
+    """The launch behind hackable_lm::hip_kv_cache_write."""
+    _no_grad_only("kv_cache_write", k, v)
+    _check_cache_tensors("cache", cache_k, cache_v, k_scale, v_scale)
+    if k.shape != v.shape or k.dim() != 4 or k.shape[2] != cache_k.shape[1]:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache of {tuple(cache_k.shape)}")
+    k, v = _cache_rows("k", k, cache_k), _cache_rows("v", v, cache_k)
+    B, T, Hkv, D = k.shape
+    starts, counts = _per_sequence("starts", starts, B, k.device), _per_sequence("counts", counts, B, k.device)
+    lib = _lib.load()
+    with _on_device(k.device):
+        rc = lib.hlm_attn_cache_write(
+            k.data_ptr(), v.data_ptr(), _row_strides(k), _row_strides(v), cache_k.data_ptr(), cache_v.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), cache_k.shape[2], _ptr(starts), int(start), _ptr(counts),
+            B, T, Hkv, D, _stream_handle(k.device),
+        )
+    _lib.check(rc, lib)
+
+
+@torch.library.custom_op("hackable_lm::hip_kv_cache_write", mutates_args=("cache_k", "cache_v", "k_scale", "v_scale"))
+def hip_kv_cache_write(
+    k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor,
+    v_scale: torch.Tensor, starts: torch.Tensor | None, start: int, counts: torch.Tensor | None,
+) -> None:
+    kv_cache_write_impl(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts)
+
+
+@hip_kv_cache_write.register_fake
+def _(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts):
+    return None
+
+
+def kv_cache_read_impl(
+    cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    starts: torch.Tensor | None, start: int, counts: torch.Tensor | None, length: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The launch behind hackable_lm::hip_kv_cache_read."""
+    if cache_k.device.type != "cuda":
+        raise RuntimeError(f"hip kv cache runs on ROCm devices only, got a cache on {cache_k.device}")
+    _check_cache_tensors("cache", cache_k, cache_v, k_scale, v_scale)
+    B, Hkv, S, D = cache_k.shape
+    if length < 0:
+        raise RuntimeError(f"length must be nonnegative, got {length}")
+    starts, counts = _per_sequence("starts", starts, B, cache_k.device), _per_sequence("counts", counts, B, cache_k.device)
+    k = torch.empty((B, length, Hkv, D), dtype=_BF16, device=cache_k.device)
+    v = torch.empty((B, length, Hkv, D), dtype=_BF16, device=cache_k.device)
+    lib = _lib.load()
+    with _on_device(cache_k.device):
+        rc = lib.hlm_attn_cache_read(
+            cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), S, k.data_ptr(), v.data_ptr(),
+            _ptr(starts), int(start), _ptr(counts), B, int(length), Hkv, D, _stream_handle(cache_k.device),
+        )
+    _lib.check(rc, lib)
+    return k, v
+
+
+@torch.library.custom_op("hackable_lm::hip_kv_cache_read", mutates_args=())
+def hip_kv_cache_read(
+    cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    starts: torch.Tensor | None, start: int, counts: torch.Tensor | None, length: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    return kv_cache_read_impl(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length)
+
+
+@hip_kv_cache_read.register_fake
+def _(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length):
+    B, Hkv, _, D = cache_k.shape
+    return (cache_k.new_empty((B, length, Hkv, D), dtype=_BF16), cache_k.new_empty((B, length, Hkv, D), dtype=_BF16))
+
+
+def cached_attn_impl(
+    q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    starts: torch.Tensor | None, start: int, counts: torch.Tensor | None, prefix_k: torch.Tensor | None,
+    prefix_v: torch.Tensor | None, prefix_k_scale: torch.Tensor | None, prefix_v_scale: torch.Tensor | None,
+    prefix_length: int, window: int, scale: float,
+) -> torch.Tensor:
+    """The launches behind hackable_lm::hip_cached_attn."""
+    _no_grad_only("cached_attention", q)
+    _check_cache_tensors("cache", cache_k, cache_v, k_scale, v_scale)
+    q = _cache_rows("q", q, cache_k)
+    B, T, H, D = q.shape
+    Hkv, S = cache_k.shape[1], cache_k.shape[2]
+    if H % Hkv != 0 or H == 0:
+        raise RuntimeError(f"query heads {H} are not a multiple of kv heads {Hkv}")
+    P = int(prefix_length) if prefix_k is not None else 0
+    if prefix_k is not None:
+        _check_cache_tensors("prefix", prefix_k, prefix_v, prefix_k_scale, prefix_v_scale)
+        if prefix_k.device != q.device or prefix_k.shape[0] != 1 or prefix_k.shape[1] != Hkv or prefix_k.shape[3] != D:
+            raise RuntimeError(f"a prefix of {tuple(prefix_k.shape)} on {prefix_k.device} does not match a cache of {tuple(cache_k.shape)}")
+    starts, counts = _per_sequence("starts", starts, B, q.device), _per_sequence("counts", counts, B, q.device)
+    o = torch.empty((B, T, H, D), dtype=_BF16, device=q.device)
+    lib = _lib.load()
+    places = (_ptr(starts), int(start), _ptr(counts))
+    nbytes = lib.hlm_attn_cached_fwd_workspace_bytes(B, T, H, Hkv, D, S, *places, P, int(window))
+    if nbytes < 0:
+        _lib.check(int(nbytes), lib)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    with _on_device(q.device):
+        rc = lib.hlm_attn_cached_fwd(
+            q.data_ptr(), _row_strides(q), o.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), S, *places, _ptr(prefix_k), _ptr(prefix_v), _ptr(prefix_k_scale), _ptr(prefix_v_scale),
+            0 if prefix_k is None else prefix_k.shape[2], P, B, T, H, Hkv, D, int(window), float(scale), _ptr(ws), nbytes,
+            _stream_handle(q.device),
+        )
+    _lib.check(rc, lib)
+    return o
+
+
+@torch.library.custom_op("hackable_lm::hip_cached_attn", mutates_args=())
+def hip_cached_attn(
+    q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    starts: torch.Tensor | None, start: int, counts: torch.Tensor | None, prefix_k: torch.Tensor | None,
+    prefix_v: torch.Tensor | None, prefix_k_scale: torch.Tensor | None, prefix_v_scale: torch.Tensor | None,
+    prefix_length: int, window: int, scale: float,
+) -> torch.Tensor:
+    return cached_attn_impl(q, cache_k, cache_v, k_scale, v_scale, starts, start, counts, prefix_k, prefix_v,
+                            prefix_k_scale, prefix_v_scale, prefix_length, window, scale)
+
+
+@hip_cached_attn.register_fake
+def _(q, cache_k, cache_v, k_scale, v_scale, starts, start, counts, prefix_k, prefix_v, prefix_k_scale, prefix_v_scale,
+      prefix_length, window, scale):
+    return q.new_empty(q.shape, dtype=_BF16)

@@ -316,6 +316,61 @@ int hlm_residual_rms_norm_fwd(const void* residual, const void* branch, void* ou
 int hlm_residual_rms_norm_bwd(const void* out, const void* grad_out, const void* grad_normed, void* grad_in,
                               int64_t rows, int n, float eps, void* stream);
 
+/*
+ * The 8-bit key/value cache of one layer: B sequences of `slots` token
+ * positions (a multiple of 64, at most 2^24), Hkv heads of D in {64, 128}.
+ *   cache_k  bytes (B, Hkv, slots, D)
+ *   cache_v  bytes (B, Hkv, slots / 64, D, 64): blocks of 64 tokens, transposed
+ *   k_scale, v_scale  fp32 (B, Hkv, slots)
+ * all contiguous and 16-byte aligned.  A row x (one token, one head) is held
+ * as bytes c + 128, c = 127 x / max|x| to the nearest (ties to even), and
+ * the scale max|x| / 127.  Rows whose largest value is below 2^-119 are held
+ * as zeros; rows with an infinity or a NaN get the scale NaN.
+ *
+ * Places: token t of sequence b lies at position starts[b] + t (int32, device
+ * memory), or start + t where starts is null; of its T tokens the first
+ * counts[b] are real (int32, device memory; null: all).  The others, and those
+ * at positions outside 0 .. slots - 1, are padding: they are not written, read
+ * as zeros, and as queries have output rows of zeros.  Places that the host
+ * knows (starts null) must fit the cache, or the call fails.
+ *
+ * hlm_attn_cache_write stores k and v, bf16 (B, T, Hkv, D) with unit D stride
+ * and {stride_b, stride_t, stride_h} element strides (multiples of 8, 16-byte
+ * aligned bases).  hlm_attn_cache_read writes them back as contiguous bf16
+ * (B, T, Hkv, D).  No counterpart in the reference, whose generation loop runs
+ * the whole prefix again for each token (lm_eval_hackable_lm.py:185-207).
+ */
+int hlm_attn_cache_write(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides, void* cache_k,
+                         void* cache_v, float* k_scale, float* v_scale, int slots, const int32_t* starts, int start,
+                         const int32_t* counts, int B, int T, int Hkv, int D, void* stream);
+int hlm_attn_cache_read(const void* cache_k, const void* cache_v, const float* k_scale, const float* v_scale, int slots,
+                        void* k, void* v, const int32_t* starts, int start, const int32_t* counts, int B, int T, int Hkv,
+                        int D, void* stream);
+
+/*
+ * Attention of T new tokens per sequence over such a cache: the query of
+ * position p sees the cached keys of positions max(0, p - window + 1) .. p
+ * (window <= 0: all of them), itself among them, so its own key is written
+ * first.  With a prefix (a cache of one sequence, prefix_slots positions, of
+ * which the first prefix_length are read; 0: none, and its pointers may be
+ * null) all sequences see the prefix at positions 0 .. prefix_length - 1 and
+ * their own tokens behind it, at prefix_length + starts[b] + t.
+ *   q  bf16 (B, T, H, D), strides as k's above;  o  bf16 (B, T, H, D), contiguous
+ * H % Hkv == 0; scale > 0; B T H <= 2^30.  ws (16-byte aligned, no
+ * initialisation needed, not shared by calls that may overlap) holds
+ * hlm_attn_cached_fwd_workspace_bytes bytes for the same sizes and places.
+ * Nothing is allocated and the host never waits.
+ */
+int hlm_attn_cached_fwd(const void* q, const int64_t* q_strides, void* o, const void* cache_k, const void* cache_v,
+                        const float* k_scale, const float* v_scale, int slots, const int32_t* starts, int start,
+                        const int32_t* counts, const void* prefix_k, const void* prefix_v, const float* prefix_k_scale,
+                        const float* prefix_v_scale, int prefix_slots, int prefix_length, int B, int T, int H, int Hkv,
+                        int D, int window, float scale, void* ws, int64_t ws_bytes, void* stream);
+/* Bytes of its workspace (0 possible); negative: an HLM_ATTN_E* code.  Reads
+ * of starts and counts only whether they are null; touches no device. */
+int64_t hlm_attn_cached_fwd_workspace_bytes(int B, int T, int H, int Hkv, int D, int slots, const int32_t* starts, int start,
+                                            const int32_t* counts, int prefix_length, int window);
+
 /* Message describing the last failed call on this thread ("" if none). */
 const char* hlm_attn_last_error(void);
 
