@@ -22,9 +22,10 @@ class KVCache:
     lengths, so one tensor of positions can serve all layers of a model, on the
     device, inside a captured graph.  Positions never written read as zeros.
 
-      k        uint8 (batch, n_kv_head, capacity, D): whole numbers + 128
-      v        uint8 (batch, n_kv_head, capacity / 64, D, 64): the same, in
-               blocks of 64 tokens, transposed
+      k        uint8 (batch, n_kv_head, capacity / 16, D / 16, 16, 16):
+               whole numbers + 128, [token / 16][dim / 16][token % 16][dim % 16]
+      v        uint8 (batch, n_kv_head, capacity / 64, D / 16, 4, 16, 16):
+               [dim / 16][token / 4 % 4][dim % 16][4 (token / 16 % 4) + token % 4]
       k_scale, v_scale  float32 (batch, n_kv_head, capacity)
 
     D is 64 or 128: other head dims are held zero-padded to the next of them,
@@ -41,8 +42,9 @@ class KVCache:
         if self.capacity > 1 << 24:
             raise RuntimeError(f"capacity {capacity} is beyond {1 << 24} tokens")
         shape = (self.batch, self.n_kv_head, self.capacity)
-        self.k = torch.empty((*shape, self.kernel_dim), dtype=torch.uint8, device=device)
-        self.v = torch.empty((*shape[:2], self.capacity // BLOCK, self.kernel_dim, BLOCK), dtype=torch.uint8, device=device)
+        pieces = self.kernel_dim // 16
+        self.k = torch.empty((*shape[:2], self.capacity // 16, pieces, 16, 16), dtype=torch.uint8, device=device)
+        self.v = torch.empty((*shape[:2], self.capacity // BLOCK, pieces, 4, 16, 16), dtype=torch.uint8, device=device)
         self.k_scale = torch.zeros(shape, dtype=torch.float32, device=device)  # a scale of zero is a row of zeros
         self.v_scale = torch.zeros(shape, dtype=torch.float32, device=device)
 

@@ -18,20 +18,20 @@
 // Layouts (v_mfma_f32_16x16x32_f16, lane l, n = l % 16, g = l / 16):
 //   A (16 x 32): row n, k = 8 g + e;  B (32 x 16): k = 8 g + e, column n;
 //   C (16 x 16): column n, rows 4 g + i.
-// Scores are formed transposed, keys by rows: tile t's row 4 g' + i is the
-// block's key 16 g' + 4 t + i, so lane (n, g) ends up with the scores of query
-// row n and the 16 consecutive keys 16 g .. 16 g + 15 in its 4 tiles.  Rounded
-// to fp16 they are the B operand of o^T = v^T p^T as they are, if its k slot
-// 8 g + e is key 16 g + 8 h + e in half h; lane (n, g) then needs the values of
-// dim n and the same 16 keys, 16 contiguous bytes of the transposed block.
+// Scores are formed transposed, keys by rows: tile t is the block's keys
+// 16 t .. 16 t + 15, so lane (n, g) ends up with the scores of query row n and
+// the 16 keys 16 t + 4 g + i.  Rounded to fp16 they are the B operand of
+// o^T = v^T p^T as they are, if its k slot 8 g + e is key 16 (2 h + e / 4) + 4 g
+// + e % 4 in half h; the A operand's lane (n, g) then needs dim n of the same 16
+// keys, which is how the cache keeps the values.
 // A score's maximum, sum and rescaling stay in the lane, but for the maximum
 // over the four g.
 //
 // Numerics.  q is scaled by a power of two to at most 2 per row and then held
 // in fp16 (exact but for values 2^-14 of the row's largest and below, whose
 // error is 2^-25 of it); whole numbers are exact; products and sums are fp32.
-// p_j vs_j is rounded to fp16 relative to the largest vs so far, 2^12 at
-// p = 1: 11 bits for p above 2^-26, and no weight above 2^-37 is lost.
+// p_j vs_j is rounded to fp16 relative to the largest vs so far, 2^11 at
+// p = 1: 11 bits for weights above 2^-25, and none above 2^-36 is lost.
 #include <utility>
 
 #include "kv_cache.h"
@@ -42,8 +42,9 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
-constexpr float kWeightTop = 4096.f;  // a probability of 1 as fp16
-// The running maximum is moved only when a score passes it by 2^3: weights
+constexpr float kWeightTop = 2048.f;  // a probability of 1 as fp16
+// The running maximum is moved only when a score passes it by 2^3, the value
+// scale that weights are relative to only when one passes it by 2: weights
 // reach 2^15, within fp16, and the sums stay where they are meanwhile.
 constexpr float kSlack = 3.f;
 
@@ -97,208 +98,167 @@ struct Keys {
   const float* vs;
 };
 
-// A query row: where it lies in q (null: padding or past the end) and which
-// keys lo .. hi of the segment it sees.
+// A query row: its sequence, token and head, and its number in o.
 struct Row {
-  const bf16* q;
-  int lo, hi;
+  int b, t, head;
+  int64_t out;
 };
 
 template <bool PREFIX>
-__device__ __forceinline__ Row row_of(const CachedAttnArgs& p, int unit, int r, int64_t& out) {
-  int bt, b, t, h;
+__device__ __forceinline__ Row row_of(const CachedAttnArgs& p, int unit, int r) {
+  Row row;
   const int rt = fast_div(r, p.div_G), g = r - rt * p.G;
+  int bt, h;
   if constexpr (PREFIX) {
     bt = rt;
-    b = fast_div(bt, p.div_T);
-    t = bt - b * p.span.T;
+    row.b = fast_div(bt, p.div_T);
+    row.t = bt - row.b * p.span.T;
     h = unit;
   } else {
-    b = unit / p.Hkv;
-    h = unit - b * p.Hkv;
-    t = rt;
-    bt = b * p.span.T + t;
+    row.b = unit / p.Hkv;
+    h = unit - row.b * p.Hkv;
+    row.t = rt;
+    bt = row.b * p.span.T + row.t;
   }
-  const int head = h * p.G + g;
-  out = (int64_t)bt * p.H + head;
-  const int pos = cache_position(span_start(p.span, b), span_count(p.span, b), t, p.own.slots);
-  Row row{nullptr, 0x7fffffff, -1};
-  if (pos < 0) return row;
-  row.q = p.q + b * p.sq[0] + t * p.sq[1] + head * p.sq[2];
-  const int64_t from = (int64_t)pos - p.window + 1;
-  if constexpr (PREFIX) {
-    const int64_t lo = from + p.P;
-    row.hi = p.P - 1;
-    row.lo = (int)min((int64_t)p.P, max((int64_t)0, lo));
-  } else {
-    row.hi = pos;
-    row.lo = (int)max((int64_t)0, from);
-  }
+  row.head = h * p.G + g;
+  row.out = (int64_t)bt * p.H + row.head;
   return row;
 }
 
-template <int D, int NT, bool PREFIX>
-__device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
-                                       bool partial, float* lds) {
-  constexpr int C = D / 64, DT = D / 16, ROWS = 16 * NT, LD = D + 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int n_rows = PREFIX ? p.B * p.span.T * p.G : p.span.T * p.G;
-  Keys s;
-  {
-    const KvCache& c = PREFIX ? p.prefix : p.own;
-    const int64_t head = (int64_t)unit * c.slots;
-    s = {c.k + head * D, c.v + head * D, c.ks + head, c.vs + head};
+// The segment's keys lo .. hi that the row sees (hi < lo: none).
+template <bool PREFIX>
+__device__ __forceinline__ void keys_seen(const CachedAttnArgs& p, const Row& row, int& lo, int& hi) {
+  lo = 0x7fffffff;
+  hi = -1;
+  const int pos = cache_position(span_start(p.span, row.b), span_count(p.span, row.b), row.t, p.own.slots);
+  if (pos < 0) return;
+  const int64_t from = (int64_t)pos - p.window + 1;
+  if constexpr (PREFIX) {
+    hi = p.P - 1;
+    lo = (int)min((int64_t)p.P, max((int64_t)0, from + p.P));
+  } else {
+    hi = pos;
+    lo = (int)max((int64_t)0, from);
   }
+}
 
-  // This lane's query rows: their keys, and q in fp16.
-  int lo[NT], hi[NT], first = 0x7fffffff, last = -1, inner_first = -1, inner_last = 0x7fffffff;
+// Lane 16 g + 4 t + i holds the scales of the block's key 16 t + 4 g + i, so
+// that row_lane<4 t + i> hands a group those of its own keys.
+__device__ __forceinline__ int lane_key(int lane) { return 16 * (lane >> 2 & 3) + 4 * (lane >> 4) + (lane & 3); }
+
+// What one wave holds of its 16 NT query rows.
+template <int D, int NT>
+struct Rows {
+  static constexpr int C = D / 64, DT = D / 16;
+  int lo[NT], hi[NT];  // the keys that this lane's rows see
+  int first, last;     // all keys that some row of the wave sees
+  int inner_first, inner_last;  // the keys that every row sees
   f16x8 q[NT][C][2];
-  float rs[NT];
+  float rs[NT];             // scale log2(e) and q's power of two
+  float mt[NT], l[NT];      // running maximum of (q.kc) ks, sum
+  float vtop;               // weights are relative to this value scale
+  f32x4 o[NT][DT];          // o^T: dims 16 d + 4 g + i of row n
+
+  // The rows r0 .. of a unit.  Queries are loaded before the places are known
+  // (of padding rows too, whose results nothing uses): both come from memory.
+  template <bool PREFIX>
+  __device__ __forceinline__ void begin(const CachedAttnArgs& p, int unit, int r0, int n_rows, int lane, bf16x8 x[NT][C][2]) {
+    const int n = lane & 15, g = lane >> 4;
+    Row row[NT];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = tile * ROWS + 16 * nt + n;
-    int64_t out;
-    Row row{nullptr, 0x7fffffff, -1};
-    if (r < n_rows) row = row_of<PREFIX>(p, unit, r, out);
-    lo[nt] = row.lo;
-    hi[nt] = row.hi;
-    if (row.hi >= row.lo) {
-      first = min(first, row.lo);
-      last = max(last, row.hi);
-      inner_first = max(inner_first, row.lo);
-      inner_last = min(inner_last, row.hi);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + 16 * nt + n;
+      row[nt] = row_of<PREFIX>(p, unit, min(r, n_rows - 1));
+      const bf16* at = p.q + row[nt].b * p.sq[0] + row[nt].t * p.sq[1] + row[nt].head * p.sq[2] + 16 * g;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[nt][c][h] = *reinterpret_cast<const bf16x8*>(at + 64 * c + 8 * h);
     }
+    first = inner_last = 0x7fffffff;
+    last = inner_first = -1;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      keys_seen<PREFIX>(p, row[nt], lo[nt], hi[nt]);
+      if (r0 + 16 * nt + n >= n_rows) hi[nt] = -1;
+      if (hi[nt] >= lo[nt]) {
+        first = min(first, lo[nt]);
+        last = max(last, hi[nt]);
+        inner_first = max(inner_first, lo[nt]);
+        inner_last = min(inner_last, hi[nt]);
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+      first = min(first, __shfl_xor(first, m));
+      last = max(last, __shfl_xor(last, m));
+      inner_first = max(inner_first, __shfl_xor(inner_first, m));
+      inner_last = min(inner_last, __shfl_xor(inner_last, m));
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
+    inner_first = __builtin_amdgcn_readfirstlane(inner_first);
+    inner_last = __builtin_amdgcn_readfirstlane(inner_last);
+  }
+
+  __device__ __forceinline__ void take_q(const CachedAttnArgs& p, const bf16x8 x[NT][C][2]) {
     typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
-    bf16x8 x[C][2];
-    int top = 0;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int nt = 0; nt < NT; ++nt) {
+      int top = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        x[c][h] = bf16x8{};
-        if (row.q != nullptr) x[c][h] = *reinterpret_cast<const bf16x8*>(row.q + 64 * c + 16 * g + 8 * h);
-        const u16x8 bits = __builtin_bit_cast(u16x8, x[c][h]);
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, (int)(bits[e] & 0x7fff));
-      }
-    top = max(top, __shfl_xor(top, 16));
-    top = max(top, __shfl_xor(top, 32));
-    const int ex = min(126, max(-120, (top >> 7) - 127));
-    const float down = __builtin_bit_cast(float, (127 - ex) << 23);
-    // kept positive and finite: a score of -infinity times it stays what it is
-    rs[nt] = fminf(3e38f, fmaxf(1e-37f, p.scale_log2 * __builtin_bit_cast(float, (127 + ex) << 23)));
+        for (int h = 0; h < 2; ++h) {
+          const u16x8 bits = __builtin_bit_cast(u16x8, x[nt][c][h]);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[nt][c][h][e] = (_Float16)((float)x[c][h][e] * down);
-  }
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) {
-    first = min(first, __shfl_xor(first, m));
-    last = max(last, __shfl_xor(last, m));
-    inner_first = max(inner_first, __shfl_xor(inner_first, m));
-    inner_last = min(inner_last, __shfl_xor(inner_last, m));
-  }
-  first = __builtin_amdgcn_readfirstlane(first);
-  last = __builtin_amdgcn_readfirstlane(last);
-  inner_first = __builtin_amdgcn_readfirstlane(inner_first);
-  inner_last = __builtin_amdgcn_readfirstlane(inner_last);
-
-  // This workgroup's blocks begin .. end - 1, shared out evenly.
-  int begin = 0, end = 0;
-  if (last >= first) {
-    const int b0 = first >> 6, blocks = (last >> 6) - b0 + 1;
-    const int per = (blocks + n_splits - 1) / n_splits;
-    begin = b0 + min(blocks, split * per);
-    end = b0 + min(blocks, split * per + per);
-  }
-
-  float mt[NT], l[NT], vtop = 0.f;  // running maximum of (q.kc) ks, sum, largest value scale
-  f32x4 o[NT][DT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    mt[nt] = -__builtin_inff();
-    l[nt] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  u32x4 kr[4][C], vr[DT];
-  float ksl = 0.f, vsl = 0.f;
-  const int key_row = 16 * (n >> 2) + (n & 3);  // + 4 t: this lane's key of tile t as an A row
-  auto load_k = [&](int blk) {
-    const uint8_t* at = s.k + (int64_t)blk * (64 * D) + key_row * D + 16 * g;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int c = 0; c < C; ++c) kr[t][c] = *reinterpret_cast<const u32x4*>(at + 4 * t * D + 64 * c);
-    ksl = s.ks[blk * 64 + lane];
-  };
-  auto load_v = [&](int blk) {
-    const uint8_t* at = s.v + (int64_t)blk * (64 * D) + n * 64 + 16 * g;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const u32x4*>(at + 16 * 64 * d);
-    vsl = s.vs[blk * 64 + lane];
-  };
-
-  int blk = begin + wave;
-  if (blk < end) {
-    load_k(blk);
-    load_v(blk);
-  }
-  for (; blk < end; blk += 4) {
-    const bool more = blk + 4 < end;
-    const int k0 = blk * 64;
-    const bool whole = k0 >= inner_first && k0 + 63 <= inner_last;  // every row sees every key
-    // scores of all rows
-    f32x4 sc[NT][4];
-    {
-      const float ks = ksl;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f16x8 kf[C][2];
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) kf[c][h] = decode8(kr[t][c][2 * h], kr[t][c][2 * h + 1]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          f32x4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) acc = mfma16(kf[c][h], q[nt][c][h], acc);
-          sc[nt][t] = acc;
+          for (int e = 0; e < 8; ++e) top = max(top, (int)(bits[e] & 0x7fff));
         }
-      }
-      if (more) load_k(blk + 4);
-      each<16>([&](auto e) {
-        const float f = row_lane<e>(ks);
+      top = max(top, __shfl_xor(top, 16));
+      top = max(top, __shfl_xor(top, 32));
+      const int ex = min(126, max(-120, (top >> 7) - 127));
+      const float down = __builtin_bit_cast(float, (127 - ex) << 23);
+      // kept positive and finite: a score of -infinity times it stays what it is
+      rs[nt] = fminf(3e38f, fmaxf(1e-37f, p.scale_log2 * __builtin_bit_cast(float, (127 + ex) << 23)));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][e / 4][e % 4] *= f;
-      });
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[nt][c][h][e] = (_Float16)((float)x[nt][c][h][e] * down);
+      mt[nt] = -__builtin_inff();
+      l[nt] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    vtop = 0.f;
+  }
+
+  // Scores sc of block k0 .. k0 + 63 (before the keys' scales; ks, vs: those of
+  // key k0 + lane_key(lane)) into weights w, updating the rows' statistics.
+  __device__ __forceinline__ void weigh(f32x4 sc[NT][4], float ks, float vs, int k0, int lane, f16x8 w[NT][2]) {
+    const int g = lane >> 4;
+    const bool whole = k0 >= inner_first && k0 + 63 <= inner_last;  // every row sees every key
+    each<16>([&](auto e) {
+      const float f = row_lane<e>(ks);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[nt][e / 4][e % 4] *= f;
+    });
     if (!whole) {  // selected, not added: masked slots may hold any scale
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = k0 + 16 * g + 4 * t + i;
-            if (key < lo[nt] || key > hi[nt]) sc[nt][t][i] = -__builtin_inff();
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + 16 * (e / 4) + 4 * g + e % 4;
+          if (key < lo[nt] || key > hi[nt]) sc[nt][e / 4][e % 4] = -__builtin_inff();
+        }
+      if (k0 + lane_key(lane) < first || k0 + lane_key(lane) > last) vs = 0.f;
     }
-    // the values' scales relative to the largest so far
-    float vs = vsl;
-    if (!whole && (k0 + lane < first || k0 + lane > last)) vs = 0.f;
-    float top = vs;
+    if (__any(vs > 2.f * vtop)) {
+      float top = vs;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
-    if (top > vtop) {
+      for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+      top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
       const float f = vtop / top;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -306,9 +266,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int ti
         for (int d = 0; d < DT; ++d) o[nt][d] *= f;
       vtop = top;
     }
-    vs = vtop > 0.f ? vs * (kWeightTop / vtop) : 0.f * vs;
-    // probabilities
-    f16x8 w[NT][2];
+    vs = vtop > 0.f ? vs * (1.f / vtop) * kWeightTop : 0.f * vs;  // 1 / vtop <= 2^126
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = sc[nt][0][0];
@@ -323,43 +281,141 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int ti
         for (int d = 0; d < DT; ++d) o[nt][d] *= alpha;
       }
       const float off = mt[nt] == -__builtin_inff() ? 0.f : -mt[nt] * rs[nt];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float pe = __builtin_amdgcn_exp2f(fmaf(sc[nt][e / 4][e % 4], rs[nt], off));
-        l[nt] += pe;
+        sum[e % 4] += pe;
         sc[nt][e / 4][e % 4] = pe;
       }
+      l[nt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    each<16>([&](auto e) {
-      const float f = row_lane<e>(vs);
+    if (whole) {
+      each<16>([&](auto e) {
+        const float f = row_lane<e>(vs);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) w[nt][e / 8][e % 8] = (_Float16)(sc[nt][e / 4][e % 4] * f);
+      });
+    } else {
+      each<16>([&](auto e) {
+        const float f = row_lane<e>(vs);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float pe = sc[nt][e / 4][e % 4];
+          w[nt][e / 8][e % 8] = (_Float16)(pe == 0.f ? 0.f : pe * f);
+        }
+      });
+    }
+  }
+
+  // The maximum in log2 units.
+  __device__ __forceinline__ float top2(int nt) const { return mt[nt] == -__builtin_inff() ? mt[nt] : mt[nt] * rs[nt]; }
+};
+
+// The head's rows of a cache.
+template <int D>
+__device__ __forceinline__ Keys keys_of(const KvCache& c, int unit) {
+  const int64_t head = (int64_t)unit * c.slots;
+  return {c.k + head * D, c.v + head * D, c.ks + head, c.vs + head};
+}
+
+// This workgroup's blocks begin .. end - 1 of the keys first .. last, shared
+// out evenly.
+__device__ __forceinline__ void share(int first, int last, int split, int n_splits, int& begin, int& end) {
+  begin = end = 0;
+  if (last < first) return;
+  const int b0 = first >> 6, blocks = (last >> 6) - b0 + 1, per = (blocks + n_splits - 1) / n_splits;
+  begin = b0 + min(blocks, split * per);
+  end = b0 + min(blocks, split * per + per);
+}
+
+// 16 NT rows, the keys shared by the four waves.
+template <int D, int NT, bool PREFIX>
+__device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
+                                             bool partial, float* lds) {
+  constexpr int C = D / 64, DT = D / 16, ROWS = 16 * NT, LD = D + 4, NW = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int n_rows = PREFIX ? p.B * p.span.T * p.G : p.span.T * p.G;
+  const Keys s = keys_of<D>(PREFIX ? p.prefix : p.own, unit);
+  Rows<D, NT> rows;
+  bf16x8 x_q[NT][C][2];
+  rows.template begin<PREFIX>(p, unit, tile * ROWS, n_rows, lane, x_q);
+  int begin, end;
+  share(rows.first, rows.last, split, n_splits, begin, end);
+
+  // Keys and values are read once: past the caches' retention (27.0 against
+  // 29.8 us for 64 sequences of up to 2048 tokens, 12 heads of 64).
+  u32x4 kr[4][C], vr[DT];
+  float ksl = 0.f, vsl = 0.f;
+  auto load_k = [&](int blk) {
+    const u32x4* at = reinterpret_cast<const u32x4*>(s.k + (int64_t)blk * (64 * D)) + lane;
+    ksl = s.ks[blk * 64 + lane_key(lane)];
+    vsl = s.vs[blk * 64 + lane_key(lane)];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < C; ++c) kr[t][c] = __builtin_nontemporal_load(at + (t * C + c) * 64);
+  };
+  auto load_v = [&](int blk) {
+    const u32x4* at = reinterpret_cast<const u32x4*>(s.v + (int64_t)blk * (64 * D)) + lane;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vr[d] = __builtin_nontemporal_load(at + 64 * d);
+  };
+
+  int blk = begin + wave;
+  if (blk < end) {
+    load_k(blk);
+    load_v(blk);
+  }
+  rows.take_q(p, x_q);
+  for (; blk < end; blk += NW) {
+    const bool more = blk + NW < end;
+    f32x4 sc[NT][4];
+    f16x8 w[NT][2];
+    const float ks = ksl, vs = vsl;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f16x8 kf[C][2];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) kf[c][h] = decode8(kr[t][c][2 * h], kr[t][c][2 * h + 1]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float pe = sc[nt][e / 4][e % 4];
-        w[nt][e / 8][e % 8] = (_Float16)(pe == 0.f ? 0.f : pe * f);
+        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) acc = mfma16(kf[c][h], rows.q[nt][c][h], acc);
+        sc[nt][t] = acc;
       }
-    });
+    }
+    if (more) load_k(blk + NW);
+    rows.weigh(sc, ks, vs, blk * 64, lane, w);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f16x8 v0 = decode8(vr[d][0], vr[d][1]), v1 = decode8(vr[d][2], vr[d][3]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        o[nt][d] = mfma16(v0, w[nt][0], o[nt][d]);
-        o[nt][d] = mfma16(v1, w[nt][1], o[nt][d]);
+        rows.o[nt][d] = mfma16(v0, w[nt][0], rows.o[nt][d]);
+        rows.o[nt][d] = mfma16(v1, w[nt][1], rows.o[nt][d]);
       }
     }
-    if (more) load_v(blk + 4);
+    if (more) load_v(blk + NW);
   }
 
-  // Join the four waves: maxima and sums, then o relative to the common maximum.
-  float* ml = lds;                   // (4, ROWS, 2)
-  float* sums = lds + 4 * ROWS * 2;  // (4, ROWS, LD)
+  // Join the waves: maxima and sums, then o relative to the common maximum.
+  float* ml = lds;                        // (NW, ROWS, 2)
+  int* real = reinterpret_cast<int*>(lds + NW * ROWS * 2);  // (ROWS)
+  float* sums = lds + NW * ROWS * 2 + ROWS;                 // (NW, ROWS, LD)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    l[nt] = sum_over_groups(l[nt]);
+    const float l = sum_over_groups(rows.l[nt]);
     if (g == 0) {
       float* at = ml + (wave * ROWS + 16 * nt + n) * 2;
-      at[0] = mt[nt] == -__builtin_inff() ? mt[nt] : mt[nt] * rs[nt];
-      at[1] = l[nt];
+      at[0] = rows.top2(nt);
+      at[1] = l;
+      if (wave == 0) real[16 * nt + n] = rows.hi[nt] >= rows.lo[nt];
     }
   }
   __syncthreads();
@@ -368,110 +424,292 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int ti
     const int r = 16 * nt + n;
     float m = ml[r * 2];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[(w * ROWS + r) * 2]);
-    const float mine = ml[(wave * ROWS + r) * 2];
-    const float f = mine == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mine - m) * (vtop / kWeightTop);
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, ml[(w * ROWS + r) * 2]);
+    const float mine = rows.top2(nt);
+    const float f = mine == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mine - m) / kWeightTop;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = o[nt][d] * f;
+      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = rows.o[nt][d] * f * rows.vtop;
   }
   __syncthreads();
-  constexpr int U = D / 8;
-  for (int i = threadIdx.x; i < ROWS * U; i += kThreads) {
+  constexpr int U = D / 4;
+  for (int i = threadIdx.x; i < ROWS * U; i += 64 * NW) {
     const int rl = i / U, u = i % U, r = tile * ROWS + rl;
     if (r >= n_rows) continue;
-    int64_t out;
-    const Row row = row_of<PREFIX>(p, unit, r, out);
-    const bool real = row.hi >= row.lo;
+    const int64_t out = row_of<PREFIX>(p, unit, r).out;
     float m = ml[rl * 2];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[(w * ROWS + rl) * 2]);
-    float sum = 0.f, x[8];
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, ml[(w * ROWS + rl) * 2]);
+    float sum = 0.f;
+    f32x4 x{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float mw = ml[(w * ROWS + rl) * 2], lw = ml[(w * ROWS + rl) * 2 + 1];
       sum += mw == -__builtin_inff() ? 0.f * lw : __builtin_amdgcn_exp2f(mw - m) * lw;
-      const f32x4 a = *reinterpret_cast<const f32x4*>(sums + (w * ROWS + rl) * LD + 8 * u);
-      const f32x4 b = *reinterpret_cast<const f32x4*>(sums + (w * ROWS + rl) * LD + 8 * u + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] += a[e];
-        x[4 + e] += b[e];
-      }
+      x += *reinterpret_cast<const f32x4*>(sums + (w * ROWS + rl) * LD + 4 * u);
     }
     if (!partial) {
-      bf16x8 y = {};
-      if (real) {
+      bf16x4 y = {};
+      if (real[rl]) {
         const float inv = 1.f / sum;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (bf16)(x[e] * inv);
+        for (int e = 0; e < 4; ++e) y[e] = (bf16)(x[e] * inv);
       }
-      *reinterpret_cast<bf16x8*>(p.o + out * D + 8 * u) = y;
+      *reinterpret_cast<bf16x4*>(p.o + out * D + 4 * u) = y;
     } else {
       const int64_t at = (int64_t)slot * ((int64_t)p.B * p.span.T * p.H) + out;
-      const bool has = real && end > begin;
+      const bool has = real[rl] && end > begin;
       if (u == 0) {
         p.part_ml[2 * at] = has ? m : -__builtin_inff();
         p.part_ml[2 * at + 1] = has ? sum : 0.f;
       }
-      if (has) {
-        *reinterpret_cast<f32x4*>(p.part_o + at * D + 8 * u) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(p.part_o + at * D + 8 * u + 4) = f32x4{x[4], x[5], x[6], x[7]};
-      }
+      if (has) *reinterpret_cast<f32x4*>(p.part_o + at * D + 4 * u) = x;
     }
   }
 }
 
-template <int D, int NT>
-constexpr int attend_lds_floats() {
-  return 4 * 16 * NT * (2 + D + 4);
+// 64 NT rows, 16 NT to a wave.  Each wave turns a quarter of a block's codes
+// into fp16 operands in LDS, in the order in which the lanes read them (1 KB to
+// an operand, one block ahead, no conflicts), and multiplies all of the block.
+template <int D, int NT, bool PREFIX>
+__device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
+                                            bool partial, float* lds) {
+  constexpr int C = D / 64, DT = D / 16, VD = DT / 4, ROWS = 64 * NT, KF = 8 * C, F = KF + 2 * DT;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int n_rows = PREFIX ? p.B * p.span.T * p.G : p.span.T * p.G;
+  const Keys s = keys_of<D>(PREFIX ? p.prefix : p.own, unit);
+  Rows<D, NT> rows;
+  bf16x8 x_q[NT][C][2];
+  const int r0 = tile * ROWS + wave * 16 * NT;
+  rows.template begin<PREFIX>(p, unit, r0, n_rows, lane, x_q);
+  int* range = reinterpret_cast<int*>(lds);
+  if (lane == 0) {
+    range[wave] = rows.first;
+    range[4 + wave] = rows.last;
+  }
+  __syncthreads();
+  int first = range[0], last = range[4];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    first = min(first, range[w]);
+    last = max(last, range[4 + w]);
+  }
+  first = __builtin_amdgcn_readfirstlane(first);
+  last = __builtin_amdgcn_readfirstlane(last);
+  int begin, end;
+  share(first, last, split, n_splits, begin, end);
+  __syncthreads();  // range is read: the operands may overwrite it
+
+  f16x8* ops = reinterpret_cast<f16x8*>(lds);  // (2, F, 64)
+  u32x4 kr[C], vr[VD];
+  float ks_next = 0.f, vs_next = 0.f;
+  auto load = [&](int blk) {
+    const u32x4* k = reinterpret_cast<const u32x4*>(s.k + (int64_t)blk * (64 * D)) + C * 64 * wave + lane;
+    const u32x4* v = reinterpret_cast<const u32x4*>(s.v + (int64_t)blk * (64 * D)) + VD * 64 * wave + lane;
+#pragma unroll
+    for (int c = 0; c < C; ++c) kr[c] = k[64 * c];
+#pragma unroll
+    for (int d = 0; d < VD; ++d) vr[d] = v[64 * d];
+  };
+  auto load_scales = [&](int blk) {
+    ks_next = s.ks[blk * 64 + lane_key(lane)];
+    vs_next = s.vs[blk * 64 + lane_key(lane)];
+  };
+  auto store = [&](int buf) {
+    f16x8* to = ops + buf * (F * 64) + lane;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) to[((wave * C + c) * 2 + h) * 64] = decode8(kr[c][2 * h], kr[c][2 * h + 1]);
+#pragma unroll
+    for (int d = 0; d < VD; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) to[(KF + (wave * VD + d) * 2 + h) * 64] = decode8(vr[d][2 * h], vr[d][2 * h + 1]);
+  };
+  if (begin < end) {
+    load(begin);
+    load_scales(begin);
+  }
+  rows.take_q(p, x_q);
+  if (begin < end) {
+    store(0);
+    if (begin + 1 < end) load(begin + 1);
+  }
+  __syncthreads();
+  for (int blk = begin; blk < end; ++blk) {
+    const int buf = (blk - begin) & 1;
+    const float ks = ks_next, vs = vs_next;
+    if (blk + 1 < end) {
+      store(buf ^ 1);
+      load_scales(blk + 1);
+      if (blk + 2 < end) load(blk + 2);
+    }
+    if (blk * 64 <= rows.last && blk * 64 + 63 >= rows.first) {
+      const f16x8* at = ops + buf * (F * 64) + lane;
+      f32x4 sc[NT][4];
+      f16x8 w[NT][2];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f16x8 kf = at[((t * C + c) * 2 + h) * 64];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) sc[nt][t] = mfma16(kf, rows.q[nt][c][h], sc[nt][t]);
+          }
+      }
+      rows.weigh(sc, ks, vs, blk * 64, lane, w);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f16x8 vf = at[(KF + d * 2 + h) * 64];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) rows.o[nt][d] = mfma16(vf, w[nt][h], rows.o[nt][d]);
+        }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float l = sum_over_groups(rows.l[nt]);
+    const int r = r0 + 16 * nt + n;
+    if (r >= n_rows) continue;
+    const int64_t out = row_of<PREFIX>(p, unit, r).out;
+    const bool real = rows.hi[nt] >= rows.lo[nt];
+    if (!partial) {
+      const float f = real ? 1.f / (l * kWeightTop) : 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        bf16x4 y = {};
+        if (real)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = (bf16)(rows.o[nt][d][i] * f * rows.vtop);
+        *reinterpret_cast<bf16x4*>(p.o + out * D + 16 * d + 4 * g) = y;
+      }
+    } else {
+      const int64_t at = (int64_t)slot * ((int64_t)p.B * p.span.T * p.H) + out;
+      const bool has = real && end > begin;
+      if (g == 0) {
+        p.part_ml[2 * at] = has ? rows.top2(nt) : -__builtin_inff();
+        p.part_ml[2 * at + 1] = has ? l : 0.f;
+      }
+      if (has)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * d + 4 * g) = rows.o[nt][d] / kWeightTop * rows.vtop;
+    }
+  }
+}
+
+// Rows of a workgroup by variant: 0: 16, the waves share the keys; 1 and 2: 64
+// and 128, the waves share the rows.
+constexpr int tile_rows(int variant) { return variant == 0 ? 16 : 64 * variant; }
+template <int D>
+constexpr int lds_floats(int variant) {
+  return variant < 0 ? 0 : variant == 0 ? 16 * (1 + 4 * (2 + D + 4)) : 2 * (8 * (D / 64) + 2 * (D / 16)) * 64 * 4;
+}
+
+template <int D, int V, bool PREFIX>
+__device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
+                                       bool partial, float* lds) {
+  if constexpr (V == 0)
+    attend_split<D, 1, PREFIX>(p, unit, tile, split, n_splits, slot, partial, lds);
+  else
+    attend_tile<D, V, PREFIX>(p, unit, tile, split, n_splits, slot, partial, lds);
 }
 
 // Workgroups in order: the prefix's items (tile slowest), then the sequences'.
-template <int D, int NT, int NTP>
+// V, VP: variants of the own keys and of the prefix (-1: none).
+template <int D, int V, int VP>
 __global__ __launch_bounds__(kThreads) void cached_attn_kernel(CachedAttnArgs p) {
-  __shared__ __align__(16) float lds[attend_lds_floats<D, (NTP > NT ? NTP : NT)>()];
+  constexpr int own_lds = lds_floats<D>(V), prefix_lds = lds_floats<D>(VP);
+  __shared__ __align__(16) float lds[prefix_lds > own_lds ? prefix_lds : own_lds];
   int id = blockIdx.x;
   const bool partial = p.own_splits + p.prefix_splits > 1;
-  if constexpr (NTP > 0) {
+  if constexpr (VP >= 0) {
     if (id < p.prefix_items) {
       const int per = p.prefix_splits * p.Hkv, tile = id / per, rest = id - tile * per, split = rest / p.Hkv;
-      attend<D, NTP, true>(p, rest - split * p.Hkv, tile, split, p.prefix_splits, split, partial, lds);
+      attend<D, VP, true>(p, rest - split * p.Hkv, tile, split, p.prefix_splits, split, partial, lds);
       return;
     }
     id -= p.prefix_items;
   }
   const int units = p.B * p.Hkv, st = id / units, unit = id - st * units;
   const int split = st / p.own_tiles, tile = st - split * p.own_tiles;
-  attend<D, NT, false>(p, unit, p.own_tiles - 1 - tile, split, p.own_splits, p.prefix_splits + split, partial, lds);
+  attend<D, V, false>(p, unit, p.own_tiles - 1 - tile, split, p.own_splits, p.prefix_splits + split, partial, lds);
 }
 
-// Joins the splits: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in the
-// order of s.  D / 4 lanes to a row.
-template <int D>
+// Joins the splits: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 4
+// lanes take a split's row, GROUPS such teams share a row's splits (in the
+// order s = team, team + GROUPS, ..), and are added in the order of the teams.
+template <int D, int GROUPS>
 __global__ __launch_bounds__(kThreads) void cached_combine_kernel(CachedAttnArgs p) {
-  constexpr int LPR = D / 4;
+  constexpr int LPR = D / 4, PER = kThreads / (LPR * GROUPS);
+  __shared__ float sums[PER][GROUPS][D + 4];
   const int64_t rows = (int64_t)p.B * p.span.T * p.H;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-  const int c = threadIdx.x % LPR, n = p.own_splits + p.prefix_splits;
-  if (row >= rows) return;
-  float m = -__builtin_inff();
-  for (int s = 0; s < n; ++s) m = fmaxf(m, p.part_ml[2 * (s * rows + row)]);
-  float sum = 0.f;
-  bool any = false;
+  const int c = threadIdx.x % LPR, team = threadIdx.x / LPR % GROUPS, rl = threadIdx.x / (LPR * GROUPS);
+  const int64_t row = (int64_t)blockIdx.x * PER + rl;
+  const int n = p.own_splits + p.prefix_splits;
+  const bool live = row < rows;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (live ? row : 0);
+  const float* po = p.part_o + (live ? row : 0) * D + 4 * c;
+  // each team over its own splits, relative to its own maximum
+  float m = -__builtin_inff(), sum = 0.f;
   f32x4 x{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n; ++s) {
-    const float ms = p.part_ml[2 * (s * rows + row)], ls = p.part_ml[2 * (s * rows + row) + 1];
-    if (ls == 0.f) continue;  // no key of this split
-    any = true;
-    const float f = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-    sum += f * ls;
-    x += *reinterpret_cast<const f32x4*>(p.part_o + (s * rows + row) * D + 4 * c) * f;
+  for (int s0 = team; s0 < n; s0 += 4 * GROUPS) {
+    float2 a[4];
+    f32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t s = min(s0 + i * GROUPS, n - 1);
+      a[i] = ml[s * rows];
+      v[i] = *reinterpret_cast<const f32x4*>(po + s * rows * D);
+      if (s0 + i * GROUPS >= n) a[i] = make_float2(-__builtin_inff(), 0.f);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, a[i].x);
+    const float f = m == top ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    x *= f;
+    sum *= f;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = a[i].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(a[i].x - m);
+      sum += w * a[i].y;
+      // a split without keys (sum 0) wrote no row: what lies there may be anything
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += a[i].y == 0.f ? 0.f : w * v[i][e];
+    }
   }
+  if constexpr (GROUPS > 1) {
+    float* to = sums[rl][team];
+    *reinterpret_cast<f32x4*>(to + 4 * c) = x;
+    if (c == 0) {
+      to[D] = m;
+      to[D + 1] = sum;
+    }
+    __syncthreads();
+    if (team != 0) return;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, sums[rl][g][D]);
+    x = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const float mg = sums[rl][g][D], w = mg == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mg - top);
+      sum += w * sums[rl][g][D + 1];
+      x += *reinterpret_cast<const f32x4*>(&sums[rl][g][4 * c]) * w;
+    }
+  }
+  if (!live) return;
   bf16x4 y = {};
-  if (any) {
+  if (sum != 0.f) {  // NaN passes
     const float inv = 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (bf16)(x[e] * inv);
@@ -479,22 +717,23 @@ __global__ __launch_bounds__(kThreads) void cached_combine_kernel(CachedAttnArgs
   *reinterpret_cast<bf16x4*>(p.o + row * D + 4 * c) = y;
 }
 
-template <int D, int NT, int NTP>
-hipError_t launch(const CachedAttnArgs& p, hipStream_t stream) {
-  const int64_t items = (int64_t)p.prefix_items + (int64_t)p.B * p.Hkv * p.own_tiles * p.own_splits;
-  hipLaunchKernelGGL((cached_attn_kernel<D, NT, NTP>), dim3((unsigned)items), dim3(kThreads), 0, stream, p);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess || p.own_splits + p.prefix_splits == 1) return err;
-  const int64_t rows = (int64_t)p.B * p.span.T * p.H, per = kThreads / (D / 4);
-  hipLaunchKernelGGL((cached_combine_kernel<D>), dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, stream, p);
+template <int D, int GROUPS>
+hipError_t combine(const CachedAttnArgs& p, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.B * p.span.T * p.H, per = kThreads / (D / 4) / GROUPS;
+  hipLaunchKernelGGL((cached_combine_kernel<D, GROUPS>), dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
-// 16-row tiles of a workgroup for n rows.
-template <int D>
-int tiles_of(int64_t rows) {
-  return rows <= 16 ? 1 : rows <= 32 || D == 128 ? 2 : 4;
+template <int D, int V, int VP>
+hipError_t launch(const CachedAttnArgs& p, hipStream_t stream) {
+  const int64_t items = (int64_t)p.prefix_items + (int64_t)p.B * p.Hkv * p.own_tiles * p.own_splits;
+  hipLaunchKernelGGL((cached_attn_kernel<D, V, VP>), dim3((unsigned)items), dim3(kThreads), 0, stream, p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || p.own_splits + p.prefix_splits == 1) return err;
+  return p.own_splits + p.prefix_splits <= 4 ? combine<D, 1>(p, stream) : combine<D, 8>(p, stream);
 }
+
+int variant_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 64 ? 1 : 2; }
 
 }  // namespace
 
@@ -503,20 +742,18 @@ int tiles_of(int64_t rows) {
 template <int D>
 int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys) {
   const int64_t own_rows = (int64_t)p.span.T * p.G, prefix_rows = own_rows * p.B;
-  const int nt = tiles_of<D>(own_rows), ntp = tiles_of<D>(prefix_rows);
-  p.own_tiles = (int)((own_rows + 16 * nt - 1) / (16 * nt));
-  const int64_t target = 1024;
-  const auto splits = [&](int64_t items, int64_t most_keys) {
-    const int64_t blocks = (most_keys + 63) / 64;
-    return (int)std::max<int64_t>(1, std::min((target + items - 1) / items, (blocks + 3) / 4));
+  const int rows = tile_rows(variant_of(own_rows)), rows_p = tile_rows(variant_of(prefix_rows));
+  p.own_tiles = (int)((own_rows + rows - 1) / rows);
+  const auto splits = [&](int64_t items, int64_t most_keys, int variant) {
+    const int64_t blocks = (most_keys + 63) / 64, least = variant ? 2 : 16, target = variant ? 768 : 512;
+    return (int)std::max<int64_t>(1, std::min((target + items - 1) / items, (blocks + least - 1) / least));
   };
-  const int64_t tokens = (16 * nt + p.G - 1) / p.G + 1, reach = (int64_t)p.window + tokens + 63;
-  p.own_splits = splits((int64_t)p.B * p.Hkv * p.own_tiles, std::min(keys, reach));
-  p.prefix_tiles = p.prefix_splits = 0;
-  p.prefix_items = 0;
+  const int64_t reach = (int64_t)p.window + (rows + p.G - 1) / p.G + 64;
+  p.own_splits = splits((int64_t)p.B * p.Hkv * p.own_tiles, std::min(keys, reach), variant_of(own_rows));
+  p.prefix_tiles = p.prefix_splits = p.prefix_items = 0;
   if (p.P > 0) {
-    p.prefix_tiles = (int)((prefix_rows + 16 * ntp - 1) / (16 * ntp));
-    p.prefix_splits = splits((int64_t)p.Hkv * p.prefix_tiles, p.P);
+    p.prefix_tiles = (int)((prefix_rows + rows_p - 1) / rows_p);
+    p.prefix_splits = splits((int64_t)p.Hkv * p.prefix_tiles, p.P, variant_of(prefix_rows));
   }
   return (int64_t)p.Hkv * p.prefix_tiles * p.prefix_splits + (int64_t)p.B * p.Hkv * p.own_tiles * p.own_splits;
 }
@@ -525,20 +762,18 @@ template <int D>
 hipError_t launch_cached_attn(CachedAttnArgs& p, hipStream_t stream) {
   p.prefix_items = p.Hkv * p.prefix_tiles * p.prefix_splits;
   const int64_t own_rows = (int64_t)p.span.T * p.G;
-  const int nt = tiles_of<D>(own_rows), ntp = p.P > 0 ? tiles_of<D>(own_rows * p.B) : 0;
-  switch (8 * nt + ntp) {
-    case 8 * 1 + 0: return launch<D, 1, 0>(p, stream);
-    case 8 * 2 + 0: return launch<D, 2, 0>(p, stream);
-    case 8 * 1 + 1: return launch<D, 1, 1>(p, stream);
-    case 8 * 1 + 2: return launch<D, 1, 2>(p, stream);
-    case 8 * 2 + 2: return launch<D, 2, 2>(p, stream);
+  const int v = variant_of(own_rows), vp = p.P > 0 ? variant_of(own_rows * p.B) : -1;
+  switch (4 * v + vp) {
+    case 4 * 0 - 1: return launch<D, 0, -1>(p, stream);
+    case 4 * 1 - 1: return launch<D, 1, -1>(p, stream);
+    case 4 * 2 - 1: return launch<D, 2, -1>(p, stream);
+    case 4 * 0 + 0: return launch<D, 0, 0>(p, stream);
+    case 4 * 0 + 1: return launch<D, 0, 1>(p, stream);
+    case 4 * 0 + 2: return launch<D, 0, 2>(p, stream);
+    case 4 * 1 + 1: return launch<D, 1, 1>(p, stream);
+    case 4 * 1 + 2: return launch<D, 1, 2>(p, stream);
+    case 4 * 2 + 2: return launch<D, 2, 2>(p, stream);
   }
-  if constexpr (D == 64) switch (8 * nt + ntp) {
-      case 8 * 4 + 0: return launch<D, 4, 0>(p, stream);
-      case 8 * 1 + 4: return launch<D, 1, 4>(p, stream);
-      case 8 * 2 + 4: return launch<D, 2, 4>(p, stream);
-      case 8 * 4 + 4: return launch<D, 4, 4>(p, stream);
-    }
   return hipErrorInvalidValue;
 }
 

@@ -33,7 +33,7 @@ hipError_t launch_lm_head_dhidden(const void* g, int64_t ldg, const void* w, int
 hipError_t launch_residual_rms_norm(const void* a, const void* b, const void* c, void* y0, void* y1, int64_t rows,
                                     int n, float eps, bool backward, hipStream_t stream);
 template <int D>
-hipError_t launch_cache_io(const CacheIoArgs& p, bool write, hipStream_t stream);
+hipError_t launch_cache_io(CacheIoArgs& p, bool write, hipStream_t stream);
 template <int D>
 int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys);
 template <int D>
@@ -651,7 +651,7 @@ int run_cache_io(bool write, const void* k, const void* v, const int64_t* k_stri
   g_last_error[0] = '\0';
   if (B < 0 || T < 0 || Hkv <= 0) return fail(HLM_ATTN_EINVAL, "bad shape B=%d T=%d Hkv=%d", B, T, Hkv);
   if (D != 64 && D != 128) return fail(HLM_ATTN_EUNSUPPORTED, "head_dim %d is not supported (64 or 128)", D);
-  if ((int64_t)B * T >= ((int64_t)1 << 31) || (int64_t)B * T * Hkv >= ((int64_t)1 << 34))
+  if ((int64_t)B * T >= ((int64_t)1 << 31) || (int64_t)B * T * Hkv >= ((int64_t)1 << 33))
     return fail(HLM_ATTN_EUNSUPPORTED, "too many rows for one launch");
   int rc = check_span(starts, start, counts, T, slots);
   if (rc) return rc;

@@ -9,14 +9,15 @@
 // below 2^-119 is held as zeros (its scale would leave the normal fp32 range);
 // one that holds an infinity or a NaN gets the scale NaN and reads as NaN.
 //
-//   keys    k  bytes (B, Hkv, S, D)
-//   values  v  bytes (B, Hkv, S / 64, D, 64): blocks of 64 tokens, transposed
+//   keys    k  bytes (B, Hkv, S / 16, D / 16, 16, 16): [token / 16][dim / 16][token % 16][dim % 16]
+//   values  v  bytes (B, Hkv, S / 64, D / 16, 4, 16, 16): blocks of 64 tokens,
+//              [dim / 16][token / 4 % 4][dim % 16][4 (token / 16) + token % 4]
 //   k_scale, v_scale  fp32 (B, Hkv, S)
 //
-// Keys and values of one head are contiguous, 64 D bytes to a 64-token block.
-// The values' blocks are transposed because the products contract q.k over D
-// and p.v over tokens: both of their matrix operands then come out of memory
-// as 16 contiguous bytes of a lane, without a pass through LDS.
+// A 64-token block of one head is 64 D contiguous bytes of either, in the order
+// in which the attention's matrix operands want them (cached_attn.hip): the
+// products contract q.k over D and p.v over tokens, and each load instruction of
+// 16 bytes a lane reads 1 KB as it lies, without a pass through LDS.
 //
 // Token t of sequence b lies at position starts[b] + t (`start` for all
 // sequences where starts is null).  Tokens t >= counts[b], and positions
@@ -29,6 +30,16 @@
 namespace hlm {
 
 constexpr int kCacheBlock = 64;  // tokens of a block
+// The byte of (token, dim) within a head's keys or values.
+template <int D>
+__device__ __forceinline__ int64_t key_byte(int token, int d) {
+  return (int64_t)(token >> 4) * (16 * D) + (d >> 4) * 256 + (token & 15) * 16 + (d & 15);
+}
+template <int D>
+__device__ __forceinline__ int64_t value_byte(int token, int d) {
+  return (int64_t)(token >> 6) * (64 * D) + (d >> 4) * 1024 + (token >> 2 & 3) * 256 + (d & 15) * 16 +
+         (token >> 4 & 3) * 4 + (token & 3);
+}
 constexpr float kCacheTiny = 1.504632769052528e-36f;  // 2^-119
 
 struct KvCache {

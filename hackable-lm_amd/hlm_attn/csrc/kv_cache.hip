@@ -16,6 +16,8 @@
 namespace hlm {
 namespace {
 
+constexpr int kBlockTokens = 16;
+
 // One row of D values over D / 8 lanes, 8 values each: the codes as two dwords
 // and the row's scale.
 template <int D>
@@ -63,11 +65,11 @@ __global__ __launch_bounds__(256) void cache_write_rows_kernel(CacheIoArgs p) {
   const int64_t head = ((int64_t)b * p.Hkv + h) * p.cache.slots;
   if (c == 0) (is_v ? p.cache.vs : p.cache.ks)[head + pos] = scale;
   if (!is_v) {
-    *reinterpret_cast<uint2*>(p.cache.k + (head + pos) * D + 8 * c) = make_uint2(code[0], code[1]);
+    *reinterpret_cast<uint2*>(p.cache.k + head * D + key_byte<D>(pos, 8 * c)) = make_uint2(code[0], code[1]);
   } else {
-    uint8_t* to = p.cache.v + (head + (pos & ~63)) * D + (pos & 63) + (8 * c) * 64;
+    uint8_t* to = p.cache.v + head * D + value_byte<D>(pos, 8 * c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) to[64 * e] = (uint8_t)(code[e / 4] >> (8 * (e % 4)));
+    for (int e = 0; e < 8; ++e) to[16 * e] = (uint8_t)(code[e / 4] >> (8 * (e % 4)));
   }
 }
 
@@ -88,11 +90,11 @@ __global__ __launch_bounds__(256) void cache_read_rows_kernel(CacheIoArgs p) {
     const float scale = (is_v ? p.cache.vs : p.cache.ks)[head + pos];
     uint8_t code[8];
     if (!is_v) {
-      *reinterpret_cast<uint2*>(code) = *reinterpret_cast<const uint2*>(p.cache.k + (head + pos) * D + 8 * c);
+      *reinterpret_cast<uint2*>(code) = *reinterpret_cast<const uint2*>(p.cache.k + head * D + key_byte<D>(pos, 8 * c));
     } else {
-      const uint8_t* from = p.cache.v + (head + (pos & ~63)) * D + (pos & 63) + (8 * c) * 64;
+      const uint8_t* from = p.cache.v + head * D + value_byte<D>(pos, 8 * c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) code[e] = from[64 * e];
+      for (int e = 0; e < 8; ++e) code[e] = from[16 * e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (bf16)((float)((int)code[e] - 128) * scale);
@@ -100,11 +102,171 @@ __global__ __launch_bounds__(256) void cache_read_rows_kernel(CacheIoArgs p) {
   *reinterpret_cast<bf16x8*>((is_v ? p.v_out : p.k_out) + row * D + 8 * c) = x;
 }
 
+// Many tokens: one workgroup per (sequence, head, 64-token block), whose image
+// is put together in LDS and moves as 16 contiguous bytes a thread.  Half of the
+// threads take the keys, half the values; a thread holds 8 dims of 4 consecutive
+// tokens.  The image's 256-byte pieces are 272 bytes apart in LDS, so that the
+// lanes of a store fall on different banks (two to a bank at most).
+template <int D>
+struct Block {
+  int64_t head;  // this head's first slot
+  int b, h, count;
+  int64_t start, first;  // of the sequence; the block's first position
+  int lo, hi;            // its tokens lo .. hi - 1 are real
+
+  __device__ __forceinline__ explicit Block(const CacheIoArgs& p) {
+    const int id = blockIdx.x, bn = id / p.Hkv;
+    h = id - bn * p.Hkv;
+    b = bn / p.blocks;
+    start = span_start(p.span, b);
+    count = span_count(p.span, b);
+    first = ((start >> 6) + (bn - b * p.blocks)) * kCacheBlock;
+    head = ((int64_t)b * p.Hkv + h) * p.cache.slots;
+    lo = hi = 0;
+    if (first < 0 || first >= p.cache.slots) return;
+    lo = (int)max((int64_t)0, start - first);
+    hi = (int)min((int64_t)kCacheBlock, start + count - first);
+  }
+};
+
+constexpr int kPiece = 272;  // bytes of LDS for 256
+// The LDS byte of byte i of a block.
+__device__ __forceinline__ int piece_byte(int i) { return (i >> 8) * kPiece + (i & 255); }
+
+// Bytes j of four dwords as one dword.
+template <int J>
+__device__ __forceinline__ unsigned gather_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  constexpr unsigned sel = (4 + J) << 8 | J;
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, sel), __builtin_amdgcn_perm(b, a, sel), 0x05040100u);
+}
+
+template <int D>
+__global__ __launch_bounds__(4 * D) void cache_write_blocks_kernel(CacheIoArgs p) {
+  constexpr int LPR = D / 8;
+  __shared__ __align__(16) uint8_t image[2][D / 4 * kPiece];
+  const Block<D> blk(p);
+  if (blk.lo >= blk.hi) return;
+  const bool is_v = threadIdx.x >= 2 * D;
+  const int u = threadIdx.x % (2 * D), c = u % LPR, quad = u / LPR;
+  const int64_t* s = is_v ? p.sv : p.sk;
+  const bf16* from = (is_v ? p.v : p.k) + blk.b * s[0] + (blk.first - blk.start) * s[1] + blk.h * s[2] + 8 * c;
+  bf16x8 x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = 4 * quad + j;
+    x[j] = bf16x8{};
+    if (i >= blk.lo && i < blk.hi) x[j] = *reinterpret_cast<const bf16x8*>(from + i * s[1]);
+  }
+  unsigned code[4][2];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = 4 * quad + j;
+    float scale;
+    encode8<D>(x[j], code[j], scale);
+    if (c == 0 && i >= blk.lo && i < blk.hi) (is_v ? p.cache.vs : p.cache.ks)[blk.head + blk.first + i] = scale;
+    if (!is_v) *reinterpret_cast<uint2*>(image[0] + piece_byte((int)key_byte<D>(i, 8 * c))) = make_uint2(code[j][0], code[j][1]);
+  }
+  if (is_v) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint8_t* to = image[1] + piece_byte((int)value_byte<D>(4 * quad, 8 * c + 4 * i));
+      *reinterpret_cast<unsigned*>(to) = gather_bytes<0>(code[0][i], code[1][i], code[2][i], code[3][i]);
+      *reinterpret_cast<unsigned*>(to + 16) = gather_bytes<1>(code[0][i], code[1][i], code[2][i], code[3][i]);
+      *reinterpret_cast<unsigned*>(to + 32) = gather_bytes<2>(code[0][i], code[1][i], code[2][i], code[3][i]);
+      *reinterpret_cast<unsigned*>(to + 48) = gather_bytes<3>(code[0][i], code[1][i], code[2][i], code[3][i]);
+    }
+  }
+  __syncthreads();
+  const int64_t base = (blk.head + blk.first) * D;
+  const bool full = blk.lo == 0 && blk.hi == kCacheBlock;
+  const int byte = 16 * threadIdx.x;  // of 64 D
+  const u32x4 kw = *reinterpret_cast<const u32x4*>(image[0] + piece_byte(byte));
+  const u32x4 vw = *reinterpret_cast<const u32x4*>(image[1] + piece_byte(byte));
+  // 16 bytes of keys are one token's
+  const int token = (byte / (16 * D)) * 16 + (byte / 16) % 16;
+  if (full || (token >= blk.lo && token < blk.hi)) *reinterpret_cast<u32x4*>(p.cache.k + base + byte) = kw;
+  if (full) {
+    *reinterpret_cast<u32x4*>(p.cache.v + base + byte) = vw;
+  } else {  // 16 bytes of values are tokens 16 t + 4 g + i, byte 4 t + i
+    const int g = byte / 256 % 4;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int i = 16 * (k / 4) + 4 * g + k % 4;
+      if (i >= blk.lo && i < blk.hi) p.cache.v[base + byte + k] = (uint8_t)(vw[k / 4] >> (8 * (k % 4)));
+    }
+  }
+}
+
+// Eight codes times a scale.
+__device__ __forceinline__ bf16x8 decode8(unsigned lo, unsigned hi, float scale) {
+  bf16x8 x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (bf16)((float)((int)(((e < 4 ? lo : hi) >> (8 * (e % 4))) & 0xff) - 128) * scale);
+  return x;
+}
+
+template <int D>
+__global__ __launch_bounds__(4 * D) void cache_read_blocks_kernel(CacheIoArgs p) {
+  constexpr int LPR = D / 8;
+  __shared__ __align__(16) uint8_t image[2][D / 4 * kPiece];
+  const Block<D> blk(p);
+  const bool is_v = threadIdx.x >= 2 * D;
+  const int u = threadIdx.x % (2 * D), c = u % LPR, quad = u / LPR;
+  const bool any = blk.lo < blk.hi;
+  uint2 kc[4];
+  float scale[4];
+  if (any) {  // a block with a real token lies in the cache, all of it
+    const int64_t base = (blk.head + blk.first) * D;
+    const int byte = 16 * threadIdx.x;
+    const u32x4 kw = *reinterpret_cast<const u32x4*>(p.cache.k + base + byte);
+    const u32x4 vw = *reinterpret_cast<const u32x4*>(p.cache.v + base + byte);
+    const f32x4 sc = *reinterpret_cast<const f32x4*>((is_v ? p.cache.vs : p.cache.ks) + blk.head + blk.first + 4 * quad);
+    *reinterpret_cast<u32x4*>(image[0] + piece_byte(byte)) = kw;
+    *reinterpret_cast<u32x4*>(image[1] + piece_byte(byte)) = vw;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) scale[j] = sc[j];
+  }
+  __syncthreads();
+  if (any && !is_v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      kc[j] = *reinterpret_cast<const uint2*>(image[0] + piece_byte((int)key_byte<D>(4 * quad + j, 8 * c)));
+  }
+  if (any && is_v) {
+    const uint8_t* from = image[1] + piece_byte((int)value_byte<D>(4 * quad, 8 * c));
+    unsigned w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const unsigned*>(from + 16 * e);
+    kc[0] = make_uint2(gather_bytes<0>(w[0], w[1], w[2], w[3]), gather_bytes<0>(w[4], w[5], w[6], w[7]));
+    kc[1] = make_uint2(gather_bytes<1>(w[0], w[1], w[2], w[3]), gather_bytes<1>(w[4], w[5], w[6], w[7]));
+    kc[2] = make_uint2(gather_bytes<2>(w[0], w[1], w[2], w[3]), gather_bytes<2>(w[4], w[5], w[6], w[7]));
+    kc[3] = make_uint2(gather_bytes<3>(w[0], w[1], w[2], w[3]), gather_bytes<3>(w[4], w[5], w[6], w[7]));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = 4 * quad + j;
+    const int64_t t = blk.first - blk.start + i;
+    if (t < 0 || t >= p.span.T) continue;
+    bf16x8 x = {};
+    if (i >= blk.lo && i < blk.hi) x = decode8(kc[j].x, kc[j].y, scale[j]);
+    *reinterpret_cast<bf16x8*>((is_v ? p.v_out : p.k_out) + (((int64_t)blk.b * p.span.T + t) * p.Hkv + blk.h) * D + 8 * c) = x;
+  }
+}
+
 }  // namespace
 
 template <int D>
-hipError_t launch_cache_io(const CacheIoArgs& p, bool write, hipStream_t stream) {
+hipError_t launch_cache_io(CacheIoArgs& p, bool write, hipStream_t stream) {
   const int64_t rows = (int64_t)p.B * p.span.T * p.Hkv;
+  p.blocks = (p.span.T + 2 * kCacheBlock - 2) / kCacheBlock;
+  if (p.span.T >= kBlockTokens) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * p.blocks)), block(4 * D);
+    if (write)
+      hipLaunchKernelGGL((cache_write_blocks_kernel<D>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((cache_read_blocks_kernel<D>), grid, block, 0, stream, p);
+    return hipGetLastError();
+  }
   const dim3 grid((unsigned)((rows + 2048 / D - 1) / (2048 / D)), 2);
   if (write)
     hipLaunchKernelGGL((cache_write_rows_kernel<D>), grid, dim3(256), 0, stream, p);
@@ -112,7 +274,7 @@ hipError_t launch_cache_io(const CacheIoArgs& p, bool write, hipStream_t stream)
     hipLaunchKernelGGL((cache_read_rows_kernel<D>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
-template hipError_t launch_cache_io<64>(const CacheIoArgs&, bool, hipStream_t);
-template hipError_t launch_cache_io<128>(const CacheIoArgs&, bool, hipStream_t);
+template hipError_t launch_cache_io<64>(CacheIoArgs&, bool, hipStream_t);
+template hipError_t launch_cache_io<128>(CacheIoArgs&, bool, hipStream_t);
 
 }  // namespace hlm

@@ -7,6 +7,8 @@
 //   forward per token).  At batch 1 and short T the kernel takes a few
 //   microseconds, so the host work around the launch decides the call rate;
 //   done in Python it costs about twice the launch.
+// * kv_cache_write, kv_cache_read, cached_attn: one generation step's calls, for
+//   the same reason.
 // * attn_train, qk_norm_rope_train, residual_rms_norm_train: the
 //   differentiable calls of a training step as C++ autograd functions.  The
 //   Python custom ops that they stand for cost 70-170 us of host time per
@@ -329,6 +331,119 @@ std::optional<std::tuple<at::Tensor, at::Tensor>> residual_rms_norm_train(const 
   return std::make_tuple(out[0], out[1]);
 }
 
+// --- the 8-bit key/value cache ----------------------------------------------------
+
+using MaybeTensor = std::optional<at::Tensor>;
+
+// A cache's sizes, or slots = 0 for tensors not laid out as KVCache's.
+struct CacheDims {
+  int64_t B = 0, Hkv = 0, slots = 0, D = 0;
+};
+CacheDims cache_dims(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs) {
+  if (k.dim() != 6 || v.dim() != 7 || ks.dim() != 3 || !plain(k) || !plain(v) || !plain(ks) || !plain(vs)) return {};
+  if (k.scalar_type() != at::kByte || v.scalar_type() != at::kByte || ks.scalar_type() != at::kFloat ||
+      vs.scalar_type() != at::kFloat)
+    return {};
+  const int64_t B = ks.size(0), Hkv = ks.size(1), S = ks.size(2), pieces = k.size(3);
+  const int64_t ksize[6] = {B, Hkv, S / 16, pieces, 16, 16}, vsize[7] = {B, Hkv, S / 64, pieces, 4, 16, 16};
+  if (S % 64 != 0 || S > INT32_MAX || k.sizes() != at::IntArrayRef(ksize, 6) || v.sizes() != at::IntArrayRef(vsize, 7) ||
+      vs.sizes() != ks.sizes())
+    return {};
+  if (!k.is_contiguous() || !v.is_contiguous() || !ks.is_contiguous() || !vs.is_contiguous() || v.device() != k.device() ||
+      ks.device() != k.device() || vs.device() != k.device())
+    return {};
+  return {B, Hkv, S, 16 * pieces};
+}
+
+// New rows that the kernels read in place, of a cache's sequences and head dim.
+bool cache_rows_ready(const at::Tensor& x, const at::Tensor& k, const CacheDims& c) {
+  if (c.slots == 0 || x.dim() != 4 || !plain(x) || x.scalar_type() != at::kBFloat16 || x.device() != k.device())
+    return false;
+  const auto n = x.sizes(), s = x.strides();
+  if (n[0] != c.B || n[3] != c.D || s[3] != 1 || n[1] > INT32_MAX || n[2] > INT32_MAX ||
+      (at::GradMode::is_enabled() && x.requires_grad()))
+    return false;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] < 0 || s[i] % 8 != 0)) return false;
+  return reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+}
+
+bool places_ready(const MaybeTensor& t, const at::Tensor& k, const CacheDims& c) {
+  return !t || (plain(*t) && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == c.B && t->is_contiguous() &&
+                t->device() == k.device());
+}
+const int32_t* places(const MaybeTensor& t) { return t ? t->data_ptr<int32_t>() : nullptr; }
+bool fits_int(int64_t x) { return x >= INT32_MIN && x <= INT32_MAX; }
+
+// Each returns false or nothing for inputs of the general path, which converts
+// or raises.
+bool kv_cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ck, const at::Tensor& cv,
+                    const at::Tensor& ks, const at::Tensor& vs, const MaybeTensor& starts, int64_t start,
+                    const MaybeTensor& counts, int64_t stream) {
+  const CacheDims c = cache_dims(ck, cv, ks, vs);
+  if (!cache_rows_ready(k, ck, c) || !cache_rows_ready(v, ck, c) || k.sizes() != v.sizes() || k.size(2) != c.Hkv ||
+      !places_ready(starts, ck, c) || !places_ready(counts, ck, c) || !fits_int(start))
+    return false;
+  const c10::DeviceGuard guard(ck.device());
+  const Strides sk(k), sv(v);
+  check(hlm_attn_cache_write(k.data_ptr(), v.data_ptr(), sk.s, sv.s, ck.data_ptr(), cv.data_ptr(), ks.data_ptr<float>(),
+                             vs.data_ptr<float>(), (int)c.slots, places(starts), (int)start, places(counts),
+                             (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3),
+                             reinterpret_cast<void*>(static_cast<uintptr_t>(stream))));
+  return true;
+}
+
+std::optional<std::tuple<at::Tensor, at::Tensor>> kv_cache_read(const at::Tensor& ck, const at::Tensor& cv,
+                                                                const at::Tensor& ks, const at::Tensor& vs,
+                                                                const MaybeTensor& starts, int64_t start,
+                                                                const MaybeTensor& counts, int64_t length, int64_t stream) {
+  const CacheDims c = cache_dims(ck, cv, ks, vs);
+  if (c.slots == 0 || !places_ready(starts, ck, c) || !places_ready(counts, ck, c) || !fits_int(start) || length < 0 ||
+      !fits_int(length))
+    return std::nullopt;
+  const c10::DeviceGuard guard(ck.device());
+  const auto options = ck.options().dtype(at::kBFloat16);
+  at::Tensor k = at::empty({c.B, length, c.Hkv, c.D}, options), v = at::empty({c.B, length, c.Hkv, c.D}, options);
+  check(hlm_attn_cache_read(ck.data_ptr(), cv.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), (int)c.slots,
+                            k.data_ptr(), v.data_ptr(), places(starts), (int)start, places(counts), (int)c.B, (int)length,
+                            (int)c.Hkv, (int)c.D, reinterpret_cast<void*>(static_cast<uintptr_t>(stream))));
+  return std::make_tuple(k, v);
+}
+
+MaybeTensor cached_attn(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& ks,
+                        const at::Tensor& vs, const MaybeTensor& starts, int64_t start, const MaybeTensor& counts,
+                        const MaybeTensor& pk, const MaybeTensor& pv, const MaybeTensor& pks, const MaybeTensor& pvs,
+                        int64_t prefix_length, int64_t window, double scale, int64_t stream) {
+  const CacheDims c = cache_dims(ck, cv, ks, vs);
+  if (!cache_rows_ready(q, ck, c) || !places_ready(starts, ck, c) || !places_ready(counts, ck, c) || !fits_int(start) ||
+      !fits_int(window) || q.size(2) == 0 || q.size(2) % c.Hkv != 0)
+    return std::nullopt;
+  const bool prefix = pk.has_value();
+  CacheDims pc;
+  if (prefix) {
+    if (!pv || !pks || !pvs || !fits_int(prefix_length)) return std::nullopt;
+    pc = cache_dims(*pk, *pv, *pks, *pvs);
+    if (pc.slots == 0 || pc.B != 1 || pc.Hkv != c.Hkv || pc.D != c.D || pk->device() != ck.device()) return std::nullopt;
+  }
+  const c10::DeviceGuard guard(ck.device());
+  const int B = (int)q.size(0), T = (int)q.size(1), H = (int)q.size(2), Hkv = (int)c.Hkv, D = (int)c.D;
+  const int S = (int)c.slots, P = prefix ? (int)prefix_length : 0;
+  const int64_t nbytes = hlm_attn_cached_fwd_workspace_bytes(B, T, H, Hkv, D, S, places(starts), (int)start,
+                                                             places(counts), P, (int)window);
+  if (nbytes < 0) check((int)nbytes);
+  at::Tensor o = at::empty({B, T, H, D}, q.options()), ws;
+  if (nbytes > 0) ws = at::empty({nbytes}, q.options().dtype(at::kByte));
+  const Strides sq(q);
+  check(hlm_attn_cached_fwd(q.data_ptr(), sq.s, o.data_ptr(), ck.data_ptr(), cv.data_ptr(), ks.data_ptr<float>(),
+                            vs.data_ptr<float>(), S, places(starts), (int)start, places(counts),
+                            prefix ? pk->data_ptr() : nullptr, prefix ? pv->data_ptr() : nullptr,
+                            prefix ? pks->data_ptr<float>() : nullptr, prefix ? pvs->data_ptr<float>() : nullptr,
+                            (int)pc.slots, P, B, T, H, Hkv, D, (int)window, (float)scale,
+                            nbytes > 0 ? ws.data_ptr() : nullptr, nbytes,
+                            reinterpret_cast<void*>(static_cast<uintptr_t>(stream))));
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_fwd, m) {
@@ -338,4 +453,11 @@ PYBIND11_MODULE(_torch_fwd, m) {
   m.def("qk_norm_rope_train", &qk_norm_rope_train, "qk_norm_rope_train(q, k, cos, sin, eps) -> (q, k), or None");
   m.def("residual_rms_norm_train", &residual_rms_norm_train,
         "residual_rms_norm_train(residual, branch, eps) -> (out, normed), or None");
+  m.def("kv_cache_write", &kv_cache_write,
+        "kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts, stream) -> whether it was done");
+  m.def("kv_cache_read", &kv_cache_read,
+        "kv_cache_read(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length, stream) -> (k, v), or None");
+  m.def("cached_attn", &cached_attn,
+        "cached_attn(q, cache_k, cache_v, k_scale, v_scale, starts, start, counts, prefix_k, prefix_v, prefix_k_scale, "
+        "prefix_v_scale, prefix_length, window, scale, stream) -> o, or None");
 }

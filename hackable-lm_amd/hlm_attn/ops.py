@@ -715,15 +715,16 @@ def _per_sequence(name: str, x: torch.Tensor | None, batch: int, device: torch.d
     return x.contiguous()
 
 
-def _check_cache_tensors(name: str, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
-    B, Hkv, S, D = k.shape
-    if (k.dtype is not torch.uint8 or v.dtype is not torch.uint8 or k_scale.dtype is not torch.float32
-            or v_scale.dtype is not torch.float32 or v.shape != (B, Hkv, S // 64, D, 64) or k_scale.shape != (B, Hkv, S)
-            or v_scale.shape != (B, Hkv, S)):
-        raise RuntimeError(f"the {name} tensors are not those of a KVCache")
-    for t in (k, v, k_scale, v_scale):
-        if t.device != k.device or not t.is_contiguous():
-            raise RuntimeError(f"the {name} tensors must be contiguous and on one device")
+def _cache_dims(name: str, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> tuple[int, int, int, int]:
+    """(B, Hkv, slots, D) of a KVCache's tensors, or raises."""
+    if k.dim() == 6 and k_scale.dim() == 3:
+        B, Hkv, S = k_scale.shape
+        D = 16 * k.shape[3]
+        if (k.dtype is torch.uint8 and v.dtype is torch.uint8 and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+                and S % 64 == 0 and k.shape == (B, Hkv, S // 16, D // 16, 16, 16) and v.shape == (B, Hkv, S // 64, D // 16, 4, 16, 16)
+                and v_scale.shape == k_scale.shape and all(t.device == k.device and t.is_contiguous() for t in (k, v, k_scale, v_scale))):
+            return B, Hkv, S, D
+    raise RuntimeError(f"the {name} tensors are not those of a KVCache on one device")
 
 
 def _row_strides(t: torch.Tensor) -> ctypes.Array:
@@ -731,14 +732,14 @@ def _row_strides(t: torch.Tensor) -> ctypes.Array:
     return _lib.strides3(t)
 
 
-def _cache_rows(name: str, t: torch.Tensor, cache_k: torch.Tensor) -> torch.Tensor:
+def _cache_rows(name: str, t: torch.Tensor, device: torch.device, B: int, D: int) -> torch.Tensor:
     """New rows (B, T, heads, D) in a layout that the cache kernels read in place, or a copy."""
     if t.device.type != "cuda":
         raise RuntimeError(f"hip kv cache runs on ROCm devices only, got {name} on {t.device}")
     if t.dtype is not _BF16 or t.dim() != 4:
         raise RuntimeError(f"hip kv cache expects bfloat16 {name} shaped (B, T, heads, D), got {t.dtype} {tuple(t.shape)}")
-    if t.device != cache_k.device or t.shape[0] != cache_k.shape[0] or t.shape[3] != cache_k.shape[3]:
-        raise RuntimeError(f"{name} {tuple(t.shape)} on {t.device} does not match a cache of {tuple(cache_k.shape)} on {cache_k.device}")
+    if t.device != device or t.shape[0] != B or t.shape[3] != D:
+        raise RuntimeError(f"{name} {tuple(t.shape)} on {t.device} does not match a cache of {B} sequences with heads of {D} on {device}")
     s = t.stride()
     fits = s[3] == 1 and not t.data_ptr() & 15 and all(n <= 1 or (x >= 0 and not x & 7) for n, x in zip(t.shape[:3], s))
     return t if fits else t.contiguous()
@@ -752,19 +753,27 @@ def kv_cache_write_impl(
     k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor,
     v_scale: torch.Tensor, starts: torch.Tensor | None, start: int, counts: torch.Tensor | None,
 ) -> None:
-    """The launch behind hackable_lm::hip_kv_cache_write."""
+    """The launch behind hackable_lm::hip_kv_cache_write.  Like its two
+    neighbours it runs as one call of the optional torch extension where the
+    inputs are as the kernels want them."""
+    ext = _lib._torch_fwd
+    if ext is None:
+        ext = _lib.torch_fwd()
+    if ext and cache_k.is_cuda:
+        if ext.kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts, _raw_stream_of(cache_k.get_device())):
+            return
     _no_grad_only("kv_cache_write", k, v)
-    _check_cache_tensors("cache", cache_k, cache_v, k_scale, v_scale)
-    if k.shape != v.shape or k.dim() != 4 or k.shape[2] != cache_k.shape[1]:
-        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache of {tuple(cache_k.shape)}")
-    k, v = _cache_rows("k", k, cache_k), _cache_rows("v", v, cache_k)
-    B, T, Hkv, D = k.shape
+    B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
+    k, v = _cache_rows("k", k, cache_k.device, B, D), _cache_rows("v", v, cache_k.device, B, D)
+    if k.shape != v.shape or k.shape[2] != Hkv:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache with {Hkv} heads")
+    T = k.shape[1]
     starts, counts = _per_sequence("starts", starts, B, k.device), _per_sequence("counts", counts, B, k.device)
     lib = _lib.load()
     with _on_device(k.device):
         rc = lib.hlm_attn_cache_write(
             k.data_ptr(), v.data_ptr(), _row_strides(k), _row_strides(v), cache_k.data_ptr(), cache_v.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), cache_k.shape[2], _ptr(starts), int(start), _ptr(counts),
+            k_scale.data_ptr(), v_scale.data_ptr(), S, _ptr(starts), int(start), _ptr(counts),
             B, T, Hkv, D, _stream_handle(k.device),
         )
     _lib.check(rc, lib)
@@ -788,10 +797,16 @@ def kv_cache_read_impl(
     starts: torch.Tensor | None, start: int, counts: torch.Tensor | None, length: int,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The launch behind hackable_lm::hip_kv_cache_read."""
+    ext = _lib._torch_fwd
+    if ext is None:
+        ext = _lib.torch_fwd()
+    if ext and cache_k.is_cuda:
+        res = ext.kv_cache_read(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length, _raw_stream_of(cache_k.get_device()))
+        if res is not None:
+            return res
     if cache_k.device.type != "cuda":
         raise RuntimeError(f"hip kv cache runs on ROCm devices only, got a cache on {cache_k.device}")
-    _check_cache_tensors("cache", cache_k, cache_v, k_scale, v_scale)
-    B, Hkv, S, D = cache_k.shape
+    B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
     if length < 0:
         raise RuntimeError(f"length must be nonnegative, got {length}")
     starts, counts = _per_sequence("starts", starts, B, cache_k.device), _per_sequence("counts", counts, B, cache_k.device)
@@ -817,7 +832,7 @@ def hip_kv_cache_read(
 
 @hip_kv_cache_read.register_fake
 def _(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length):
-    B, Hkv, _, D = cache_k.shape
+    B, Hkv, D = cache_k.shape[0], cache_k.shape[1], 16 * cache_k.shape[3]
     return (cache_k.new_empty((B, length, Hkv, D), dtype=_BF16), cache_k.new_empty((B, length, Hkv, D), dtype=_BF16))
 
 
@@ -828,18 +843,26 @@ def cached_attn_impl(
     prefix_length: int, window: int, scale: float,
 ) -> torch.Tensor:
     """The launches behind hackable_lm::hip_cached_attn."""
+    ext = _lib._torch_fwd
+    if ext is None:
+        ext = _lib.torch_fwd()
+    if ext and cache_k.is_cuda:
+        res = ext.cached_attn(q, cache_k, cache_v, k_scale, v_scale, starts, start, counts, prefix_k, prefix_v, prefix_k_scale,
+                              prefix_v_scale, prefix_length, window, scale, _raw_stream_of(cache_k.get_device()))
+        if res is not None:
+            return res
     _no_grad_only("cached_attention", q)
-    _check_cache_tensors("cache", cache_k, cache_v, k_scale, v_scale)
-    q = _cache_rows("q", q, cache_k)
-    B, T, H, D = q.shape
-    Hkv, S = cache_k.shape[1], cache_k.shape[2]
+    B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
+    q = _cache_rows("q", q, cache_k.device, B, D)
+    T, H = q.shape[1], q.shape[2]
     if H % Hkv != 0 or H == 0:
         raise RuntimeError(f"query heads {H} are not a multiple of kv heads {Hkv}")
-    P = int(prefix_length) if prefix_k is not None else 0
+    P = prefix_slots = 0
     if prefix_k is not None:
-        _check_cache_tensors("prefix", prefix_k, prefix_v, prefix_k_scale, prefix_v_scale)
-        if prefix_k.device != q.device or prefix_k.shape[0] != 1 or prefix_k.shape[1] != Hkv or prefix_k.shape[3] != D:
-            raise RuntimeError(f"a prefix of {tuple(prefix_k.shape)} on {prefix_k.device} does not match a cache of {tuple(cache_k.shape)}")
+        P = int(prefix_length)
+        pb, ph, prefix_slots, pd = _cache_dims("prefix", prefix_k, prefix_v, prefix_k_scale, prefix_v_scale)
+        if prefix_k.device != q.device or (pb, ph, pd) != (1, Hkv, D):
+            raise RuntimeError(f"a prefix of {pb} sequences, {ph} heads of {pd} on {prefix_k.device} does not match a cache with {Hkv} heads of {D} on {q.device}")
     starts, counts = _per_sequence("starts", starts, B, q.device), _per_sequence("counts", counts, B, q.device)
     o = torch.empty((B, T, H, D), dtype=_BF16, device=q.device)
     lib = _lib.load()
@@ -852,7 +875,7 @@ def cached_attn_impl(
         rc = lib.hlm_attn_cached_fwd(
             q.data_ptr(), _row_strides(q), o.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), S, *places, _ptr(prefix_k), _ptr(prefix_v), _ptr(prefix_k_scale), _ptr(prefix_v_scale),
-            0 if prefix_k is None else prefix_k.shape[2], P, B, T, H, Hkv, D, int(window), float(scale), _ptr(ws), nbytes,
+            prefix_slots, P, B, T, H, Hkv, D, int(window), float(scale), _ptr(ws), nbytes,
             _stream_handle(q.device),
         )
     _lib.check(rc, lib)

@@ -319,8 +319,10 @@ int hlm_residual_rms_norm_bwd(const void* out, const void* grad_out, const void*
 /*
  * The 8-bit key/value cache of one layer: B sequences of `slots` token
  * positions (a multiple of 64, at most 2^24), Hkv heads of D in {64, 128}.
- *   cache_k  bytes (B, Hkv, slots, D)
- *   cache_v  bytes (B, Hkv, slots / 64, D, 64): blocks of 64 tokens, transposed
+ *   cache_k  bytes (B, Hkv, slots / 16, D / 16, 16, 16):
+ *            [token / 16][dim / 16][token % 16][dim % 16]
+ *   cache_v  bytes (B, Hkv, slots / 64, D / 16, 4, 16, 16):
+ *            [token / 64][dim / 16][token / 4 % 4][dim % 16][4 (token / 16 % 4) + token % 4]
  *   k_scale, v_scale  fp32 (B, Hkv, slots)
  * all contiguous and 16-byte aligned.  A row x (one token, one head) is held
  * as bytes c + 128, c = 127 x / max|x| to the nearest (ties to even), and

@@ -27,8 +27,11 @@ def _rand(g, *shape, scale=1.0):
 
 def plain_of(cache) -> tuple:
     """The device cache's contents as plain ones: (codes, scales) of k and of v."""
-    k = cache.k.cpu().long() - 128
-    v = cache.v.cpu().long().transpose(3, 4).reshape(cache.k.shape) - 128
+    B, Hkv, S, D = cache.batch, cache.n_kv_head, cache.capacity, cache.kernel_dim
+    k = cache.k.cpu().long() - 128  # token / 16, dim / 16, token % 16, dim % 16
+    k = k.permute(0, 1, 2, 4, 3, 5).reshape(B, Hkv, S, D)
+    v = cache.v.cpu().long().view(B, Hkv, S // 64, D // 16, 4, 16, 4, 4) - 128  # block, dim / 16, g, dim % 16, t, i: token 16 t + 4 g + i
+    v = v.permute(0, 1, 2, 6, 4, 7, 3, 5).reshape(B, Hkv, S, D)
     return (k, cache.k_scale.cpu().double()), (v, cache.v_scale.cpu().double())
 
 
@@ -208,7 +211,7 @@ def test_masked_slots_may_hold_anything(D, T, window):
         dead = list(range(s + T, 192)) + (list(range(0, max(0, s - window + 1))) if window else [])
         cache.k_scale[b, :, dead] = float("nan")
         cache.v_scale[b, :, dead] = float("nan")
-        cache.k[b, :, dead] = 255
+        cache.k[b, :, [i for i in range(192 // 16) if all(p in dead for p in range(16 * i, 16 * i + 16))]] = 255
     out = hlm_attn.cached_attention_hip(q.cuda(), cache, int32(starts), None, window)
     assert torch.equal(out, clean)
     check_attention(out, q, k, v, starts, [T] * B, window)
@@ -245,6 +248,24 @@ def test_scales_far_apart_and_one_key_that_takes_it_all(D):
     big = (q.float() * 1e20).bfloat16()
     out = hlm_attn.cached_attention_hip(big.cuda(), cache, S - 5, scale=1e-20)
     check_attention(out, big, kp, vp, [S - 5], [5], scale=1e-20)
+
+
+@pytest.mark.parametrize("T", [1, 30, 70])
+def test_values_at_the_ends_of_the_range(T):
+    g = torch.Generator().manual_seed(2)
+    D, S = 64, 256
+    for size in (2.0**-118, 2.0**100):
+        v = (torch.randn(1, S, 1, D, generator=g) * size).bfloat16()
+        v[0, :, 0, 0] = size  # no row below 2^-119
+        cache, (kp, vp) = filled(g, 1, S, 1, D, None, v)
+        q = _rand(g, 1, T, 2, D)
+        out = hlm_attn.cached_attention_hip(q.cuda(), cache, S - T)
+        o, _, _ = oracle.attention(q, kp, vp, [S - T], [T])
+        # outputs below the smallest normal bf16 may come out as zeros
+        assert ((out.double().cpu() - o).abs() <= 2.0**-6 * size + 2.0**-125).all()
+        assert (out[..., 0].double().cpu() / size - 1).abs().max() <= 2.0**-7
+    zeros = hlm_attn.KVCache(1, S, 1, D)  # all scales zero
+    assert not hlm_attn.cached_attention_hip(_rand(g, 1, T, 2, D).cuda(), zeros, S - T).any()
 
 
 def test_many_small_weights_are_not_lost():
