@@ -152,12 +152,19 @@ def _inputs(case, seed):
     return s
 
 
-def _hlm():
-    if os.path.abspath("hackable-lm_amd") not in sys.path:
-        sys.path.insert(0, os.path.abspath("hackable-lm_amd"))
-    import hlm_attn
+_package = None
 
-    return hlm_attn
+
+def _hlm():
+    """The framework's package, imported once as a user's program does."""
+    global _package
+    if _package is None:
+        if os.path.abspath("hackable-lm_amd") not in sys.path:
+            sys.path.insert(0, os.path.abspath("hackable-lm_amd"))
+        import hlm_attn
+
+        _package = hlm_attn
+    return _package
 
 
 def _cache_of(k, v, capacity):
