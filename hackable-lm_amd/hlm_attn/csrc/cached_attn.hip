@@ -32,6 +32,7 @@
 // error is 2^-25 of it); whole numbers are exact; products and sums are fp32.
 // p_j vs_j is rounded to fp16 relative to the largest vs so far, 2^11 at
 // p = 1: 11 bits for weights above 2^-25, and none above 2^-36 is lost.
+#include <cmath>
 #include <utility>
 
 #include "kv_cache.h"
@@ -128,7 +129,7 @@ __device__ __forceinline__ Row row_of(const CachedAttnArgs& p, int unit, int r) 
 // The segment's keys lo .. hi that the row sees (hi < lo: none).
 template <bool PREFIX>
 __device__ __forceinline__ void keys_seen(const CachedAttnArgs& p, const Row& row, int& lo, int& hi) {
-  lo = 0x7fffffff;
+  lo = 0;
   hi = -1;
   const int pos = cache_position(span_start(p.span, row.b), span_count(p.span, row.b), row.t, p.own.slots);
   if (pos < 0) return;
@@ -156,7 +157,7 @@ struct Rows {
   f16x8 q[NT][C][2];
   float rs[NT];             // scale log2(e) and q's power of two
   float mt[NT], l[NT];      // running maximum of (q.kc) ks, sum
-  float vtop;               // weights are relative to this value scale
+  float vtop, per_vtop;     // weights are relative to this value scale (0: none yet); its inverse
   f32x4 o[NT][DT];          // o^T: dims 16 d + 4 g + i of row n
 
   // The rows r0 .. of a unit.  Queries are loaded before the places are known
@@ -180,7 +181,10 @@ struct Rows {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       keys_seen<PREFIX>(p, row[nt], lo[nt], hi[nt]);
-      if (r0 + 16 * nt + n >= n_rows) hi[nt] = -1;
+      if (r0 + 16 * nt + n >= n_rows || hi[nt] < lo[nt]) {
+        lo[nt] = 0;
+        hi[nt] = -1;
+      }
       if (hi[nt] >= lo[nt]) {
         first = min(first, lo[nt]);
         last = max(last, hi[nt]);
@@ -231,7 +235,7 @@ struct Rows {
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    vtop = 0.f;
+    vtop = per_vtop = 0.f;
   }
 
   // Scores sc of block k0 .. k0 + 63 (before the keys' scales; ks, vs: those of
@@ -246,12 +250,12 @@ struct Rows {
     });
     if (!whole) {  // selected, not added: masked slots may hold any scale
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        const unsigned from = k0 + 4 * g - lo[nt], seen = max(0, hi[nt] - lo[nt] + 1);  // lo = 0 where hi < lo
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = k0 + 16 * (e / 4) + 4 * g + e % 4;
-          if (key < lo[nt] || key > hi[nt]) sc[nt][e / 4][e % 4] = -__builtin_inff();
-        }
+        for (int e = 0; e < 16; ++e)
+          if (from + (16 * (e / 4) + e % 4) >= seen) sc[nt][e / 4][e % 4] = -__builtin_inff();
+      }
       if (k0 + lane_key(lane) < first || k0 + lane_key(lane) > last) vs = 0.f;
     }
     if (__any(vs > 2.f * vtop)) {
@@ -265,8 +269,9 @@ struct Rows {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[nt][d] *= f;
       vtop = top;
+      per_vtop = 1.f / top;  // <= 2^126: kWeightTop times it may be beyond fp32
     }
-    vs = vtop > 0.f ? vs * (1.f / vtop) * kWeightTop : 0.f * vs;  // 1 / vtop <= 2^126
+    vs = vs * per_vtop * kWeightTop;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = sc[nt][0][0];
@@ -733,37 +738,83 @@ hipError_t launch(const CachedAttnArgs& p, hipStream_t stream) {
   return p.own_splits + p.prefix_splits <= 4 ? combine<D, 1>(p, stream) : combine<D, 8>(p, stream);
 }
 
-int variant_of(int64_t rows) { return rows <= 16 ? 0 : rows <= 64 ? 1 : 2; }
+// How `rows` query rows of each of `units` (head, keys) pairs are cut into tiles
+// and their keys, `blocks` of 64, into splits: the choice with the least time
+// by a model in microseconds, fitted on an MI355X.
+//  * Variant 0 reads keys at 4.8 TB/s on all 256 CUs, on a share x of them at
+//    x (2 - x) of that, and takes 0.8 (head dim 64) or 1.4 for each round of its
+//    four waves.
+//  * Variants 1 and 2 take 1.0 or 1.15 for a block (1.15, 1.65 at head dim 128)
+//    while a CU has one or two workgroups, then 0.45 or 0.75 (0.8, 1.3) a
+//    workgroup: the larger tile costs less a row, the smaller spreads better.
+//  * Partial sums cost 3.0 for the second kernel and are written and read at
+//    4.5 TB/s.
+struct Split {
+  int variant, tiles, splits;
+};
+
+template <int D>
+Split choose(int64_t rows, int64_t units, int64_t blocks, int64_t all_rows, bool joined) {
+  Split best{0, 1, 1};
+  double least = 1e300;
+  const double row_us = (D + 2) * 8 / 4.5e6;
+  for (int v = rows <= 16 ? 0 : 1; v <= (rows <= 16 ? 0 : rows <= 64 ? 1 : 2); ++v) {
+    const int64_t tiles = (rows + tile_rows(v) - 1) / tile_rows(v), items = units * tiles;
+    for (int n : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+      if (n > blocks && n > 1) break;
+      const double per = (double)((blocks + n - 1) / n), wg = (double)(items * n), q = std::ceil(wg / 256);
+      double t;
+      if (v == 0) {
+        const double bytes = (double)items * blocks * (128 * (D + 4));
+        const double share = std::min(1.0, wg / 256);
+        const double rounds = std::ceil(per / 4) * std::max(1.0, q / (D == 64 ? 4 : 2));
+        t = std::max(rounds * (D == 64 ? 0.8 : 1.4), bytes / (4.8e6 * share * (2 - share)));
+      } else {
+        const double one = D == 64 ? (v == 1 ? 1.0 : 1.15) : (v == 1 ? 1.15 : 1.65);
+        const double more = D == 64 ? (v == 1 ? 0.45 : 0.75) : (v == 1 ? 0.8 : 1.3);
+        t = per * std::max(one, more * q);
+      }
+      if (n > 1 || joined) t += (joined ? 0.0 : 3.0) + n * (double)all_rows * row_us;
+      if (t < 0.97 * least) {  // a later choice needs to be clearly better
+        least = t;
+        best = {v, (int)tiles, n};
+      }
+    }
+  }
+  return best;
+}
 
 }  // namespace
 
-// Row tiles, splits and work items of a problem.  `keys` bounds the own keys
-// that a sequence holds; the plan only decides how the work is shared out.
+// Variants, tiles, splits and work items of a problem.  `keys` bounds the own
+// keys that a sequence holds; the plan only decides how the work is shared out.
 template <int D>
 int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys) {
-  const int64_t own_rows = (int64_t)p.span.T * p.G, prefix_rows = own_rows * p.B;
-  const int rows = tile_rows(variant_of(own_rows)), rows_p = tile_rows(variant_of(prefix_rows));
-  p.own_tiles = (int)((own_rows + rows - 1) / rows);
-  const auto splits = [&](int64_t items, int64_t most_keys, int variant) {
-    const int64_t blocks = (most_keys + 63) / 64, least = variant ? 2 : 16, target = variant ? 768 : 512;
-    return (int)std::max<int64_t>(1, std::min((target + items - 1) / items, (blocks + least - 1) / least));
-  };
-  const int64_t reach = (int64_t)p.window + (rows + p.G - 1) / p.G + 64;
-  p.own_splits = splits((int64_t)p.B * p.Hkv * p.own_tiles, std::min(keys, reach), variant_of(own_rows));
-  p.prefix_tiles = p.prefix_splits = p.prefix_items = 0;
+  const int64_t rows = (int64_t)p.span.T * p.G, units = (int64_t)p.B * p.Hkv, all = (int64_t)p.B * p.span.T * p.H;
+  const int64_t reach = std::min(keys, (int64_t)p.window + p.span.T + 64);
+  const Split own = choose<D>(rows, units, (reach + 63) / 64, all, p.P > 0);
+  p.variant = own.variant;
+  p.own_tiles = own.tiles;
+  p.own_splits = own.splits;
+  p.prefix_variant = -1;
+  p.prefix_tiles = p.prefix_splits = 0;
   if (p.P > 0) {
-    p.prefix_tiles = (int)((prefix_rows + rows_p - 1) / rows_p);
-    p.prefix_splits = splits((int64_t)p.Hkv * p.prefix_tiles, p.P, variant_of(prefix_rows));
+    const int64_t seen = std::min<int64_t>(p.P, p.window);  // own tokens stand behind the prefix
+    Split pre = choose<D>(rows * p.B, p.Hkv, (seen + 63) / 64 + 1, all, true);
+    // one kernel for both: 128-row tiles of a sequence's rows need them of the prefix's
+    if (pre.variant < own.variant) pre.variant = own.variant, pre.tiles = (int)((rows * p.B + 127) / 128);
+    p.prefix_variant = pre.variant;
+    p.prefix_tiles = pre.tiles;
+    p.prefix_splits = pre.splits;
   }
-  return (int64_t)p.Hkv * p.prefix_tiles * p.prefix_splits + (int64_t)p.B * p.Hkv * p.own_tiles * p.own_splits;
+  const int64_t prefix_items = (int64_t)p.Hkv * p.prefix_tiles * p.prefix_splits;
+  p.prefix_items = (int)prefix_items;
+  return prefix_items + units * p.own_tiles * p.own_splits;
 }
 
 template <int D>
-hipError_t launch_cached_attn(CachedAttnArgs& p, hipStream_t stream) {
-  p.prefix_items = p.Hkv * p.prefix_tiles * p.prefix_splits;
-  const int64_t own_rows = (int64_t)p.span.T * p.G;
-  const int v = variant_of(own_rows), vp = p.P > 0 ? variant_of(own_rows * p.B) : -1;
-  switch (4 * v + vp) {
+hipError_t launch_cached_attn(const CachedAttnArgs& p, hipStream_t stream) {
+  switch (4 * p.variant + p.prefix_variant) {
     case 4 * 0 - 1: return launch<D, 0, -1>(p, stream);
     case 4 * 1 - 1: return launch<D, 1, -1>(p, stream);
     case 4 * 2 - 1: return launch<D, 2, -1>(p, stream);
@@ -779,7 +830,7 @@ hipError_t launch_cached_attn(CachedAttnArgs& p, hipStream_t stream) {
 
 template int64_t plan_cached_attn<64>(CachedAttnArgs&, int64_t);
 template int64_t plan_cached_attn<128>(CachedAttnArgs&, int64_t);
-template hipError_t launch_cached_attn<64>(CachedAttnArgs&, hipStream_t);
-template hipError_t launch_cached_attn<128>(CachedAttnArgs&, hipStream_t);
+template hipError_t launch_cached_attn<64>(const CachedAttnArgs&, hipStream_t);
+template hipError_t launch_cached_attn<128>(const CachedAttnArgs&, hipStream_t);
 
 }  // namespace hlm

@@ -37,7 +37,7 @@ hipError_t launch_cache_io(CacheIoArgs& p, bool write, hipStream_t stream);
 template <int D>
 int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys);
 template <int D>
-hipError_t launch_cached_attn(CachedAttnArgs& p, hipStream_t stream);
+hipError_t launch_cached_attn(const CachedAttnArgs& p, hipStream_t stream);
 }  // namespace hlm
 
 namespace {

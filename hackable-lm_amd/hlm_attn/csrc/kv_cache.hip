@@ -18,10 +18,10 @@ namespace {
 
 constexpr int kBlockTokens = 16;
 
-// One row of D values over D / 8 lanes, 8 values each: the codes as two dwords
-// and the row's scale.
+// One row of D values over D / 8 lanes, 8 values each: dwords whose last byte is
+// the code, and the row's scale.
 template <int D>
-__device__ __forceinline__ void encode8(const bf16x8& x, unsigned code[2], float& scale) {
+__device__ __forceinline__ void encode8(const bf16x8& x, unsigned u[8], float& scale) {
   typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
   const u16x8 bits = __builtin_bit_cast(u16x8, x);
   int top = 0;  // as bits, so that a NaN is the largest
@@ -35,12 +35,14 @@ __device__ __forceinline__ void encode8(const bf16x8& x, unsigned code[2], float
   if (fmaf(r, a, -127.f) < 0.f && r > 0.f) r = __builtin_bit_cast(float, __builtin_bit_cast(int, r) + 1);
   scale = !finite ? __builtin_nanf("") : tiny ? 0.f : a / 127.f;
   // x r + 1.5 2^23 + 128: the sum's last bits are the whole number + 128
-  unsigned u[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    u[e] = __builtin_bit_cast(unsigned, fmaf(finite ? (float)x[e] : 0.f, r, 12582912.f + 128.f)) & 0xff;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) code[i] = u[4 * i] | u[4 * i + 1] << 8 | u[4 * i + 2] << 16 | u[4 * i + 3] << 24;
+    u[e] = __builtin_bit_cast(unsigned, fmaf(finite ? (float)x[e] : 0.f, r, 12582912.f + 128.f));
+}
+
+// The last bytes of four dwords as one.
+__device__ __forceinline__ unsigned last_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
 }
 
 // One row to D / 8 lanes; a workgroup takes 2048 / D rows of k or of v
@@ -59,17 +61,18 @@ __global__ __launch_bounds__(256) void cache_write_rows_kernel(CacheIoArgs p) {
   if (pos < 0) return;
   const int64_t* s = is_v ? p.sv : p.sk;
   const bf16x8 x = *reinterpret_cast<const bf16x8*>((is_v ? p.v : p.k) + b * s[0] + t * s[1] + h * s[2] + 8 * c);
-  unsigned code[2];
+  unsigned u[8];
   float scale;
-  encode8<D>(x, code, scale);
+  encode8<D>(x, u, scale);
   const int64_t head = ((int64_t)b * p.Hkv + h) * p.cache.slots;
   if (c == 0) (is_v ? p.cache.vs : p.cache.ks)[head + pos] = scale;
   if (!is_v) {
-    *reinterpret_cast<uint2*>(p.cache.k + head * D + key_byte<D>(pos, 8 * c)) = make_uint2(code[0], code[1]);
+    *reinterpret_cast<uint2*>(p.cache.k + head * D + key_byte<D>(pos, 8 * c)) =
+        make_uint2(last_bytes(u[0], u[1], u[2], u[3]), last_bytes(u[4], u[5], u[6], u[7]));
   } else {
     uint8_t* to = p.cache.v + head * D + value_byte<D>(pos, 8 * c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) to[16 * e] = (uint8_t)(code[e / 4] >> (8 * (e % 4)));
+    for (int e = 0; e < 8; ++e) to[16 * e] = (uint8_t)u[e];
   }
 }
 
@@ -157,24 +160,26 @@ __global__ __launch_bounds__(4 * D) void cache_write_blocks_kernel(CacheIoArgs p
     x[j] = bf16x8{};
     if (i >= blk.lo && i < blk.hi) x[j] = *reinterpret_cast<const bf16x8*>(from + i * s[1]);
   }
-  unsigned code[4][2];
+  unsigned u4[4][8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int i = 4 * quad + j;
     float scale;
-    encode8<D>(x[j], code[j], scale);
+    encode8<D>(x[j], u4[j], scale);
     if (c == 0 && i >= blk.lo && i < blk.hi) (is_v ? p.cache.vs : p.cache.ks)[blk.head + blk.first + i] = scale;
-    if (!is_v) *reinterpret_cast<uint2*>(image[0] + piece_byte((int)key_byte<D>(i, 8 * c))) = make_uint2(code[j][0], code[j][1]);
   }
-  if (is_v) {
+  if (!is_v) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint8_t* to = image[1] + piece_byte((int)value_byte<D>(4 * quad, 8 * c + 4 * i));
-      *reinterpret_cast<unsigned*>(to) = gather_bytes<0>(code[0][i], code[1][i], code[2][i], code[3][i]);
-      *reinterpret_cast<unsigned*>(to + 16) = gather_bytes<1>(code[0][i], code[1][i], code[2][i], code[3][i]);
-      *reinterpret_cast<unsigned*>(to + 32) = gather_bytes<2>(code[0][i], code[1][i], code[2][i], code[3][i]);
-      *reinterpret_cast<unsigned*>(to + 48) = gather_bytes<3>(code[0][i], code[1][i], code[2][i], code[3][i]);
+    for (int j = 0; j < 4; ++j) {
+      const unsigned* w = u4[j];
+      *reinterpret_cast<uint2*>(image[0] + piece_byte((int)key_byte<D>(4 * quad + j, 8 * c))) =
+          make_uint2(last_bytes(w[0], w[1], w[2], w[3]), last_bytes(w[4], w[5], w[6], w[7]));
     }
+  } else {
+    uint8_t* to = image[1] + piece_byte((int)value_byte<D>(4 * quad, 8 * c));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<unsigned*>(to + 16 * e) = last_bytes(u4[0][e], u4[1][e], u4[2][e], u4[3][e]);
   }
   __syncthreads();
   const int64_t base = (blk.head + blk.first) * D;
