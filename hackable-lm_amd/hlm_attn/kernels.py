@@ -352,6 +352,8 @@ def _places(starts: torch.Tensor | int) -> tuple[torch.Tensor | None, int]:
 
 def _head_padded(x: torch.Tensor, cache: "KVCache", name: str) -> torch.Tensor:
     """x as bf16 with the cache's kernel head dim, zero-padded where head_dim is none."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"the hip kv cache has no backward, and {name} requires grad: call it under torch.no_grad()")
     if x.dim() != 4 or x.shape[-1] != cache.head_dim:
         raise RuntimeError(f"{name} {tuple(x.shape)} does not have 4 dims with heads of {cache.head_dim}")
     if x.dtype is not torch.bfloat16:
@@ -376,8 +378,8 @@ def kv_cache_write_hip(
     other than bf16 are rounded to it first.  No backward: tensors that require
     grad are refused outside torch.no_grad()."""
     ops = _ops or _load_ops()
-    if k.shape[-1] != cache.head_dim or v.shape != k.shape:
-        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache with heads of {cache.head_dim}")
+    if v.shape != k.shape:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
     k, v = _head_padded(k, cache, "k"), _head_padded(v, cache, "v")
     run = ops.kv_cache_write_impl if ops.direct_call_ok(k, v) else ops.hip_kv_cache_write
     run(k, v, *cache.tensors(), *_places(starts), counts)

@@ -13,6 +13,10 @@ QKVProjection mirrors model.py:76-126: the fused q/k/v projection, then the
 q/k RMSNorm + partial RoPE producer; `fwd_hip` is `fwd_triton` with the HIP
 producer in place of the Triton one, fed the same views and rotary tables.
 
+Generation over a cache has no counterpart in the reference:
+AttentionCore.forward_cached, with the tokens' rotary tables from
+RotaryEmbedding.at handed to QKVProjection.
+
 AttentionCore routes CPU tensors to `fwd_torch`, the reference's dense math
 (model.py:170, :176-196 with kernels.py:785-800), as the reference does;
 attention_backend="torch" selects it on any device.  The hip backend never
@@ -27,6 +31,7 @@ import torch
 from torch import nn
 
 from . import kernels
+from .cache import KVCache
 from .config import (
     attention_window_size,
     layer_attention_window,
@@ -87,6 +92,14 @@ class RotaryEmbedding(nn.Module):
             self._cached_len = seq_len
         return self._cos[:, :, :seq_len].to(dtype=dtype), self._sin[:, :, :seq_len].to(dtype=dtype)
 
+    def at(self, positions: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        """The same tables' rows for positions (B, T), as (B, T, R): tokens that
+        continue a cache, each sequence at a place of its own.  One pair serves
+        all layers of a step."""
+        angles = positions.to(torch.float32)[..., None] * self.inv_freq.to(positions.device)
+        angles = torch.cat((angles, angles), dim=-1)
+        return angles.cos().to(dtype=dtype), angles.sin().to(dtype=dtype)
+
 
 class QKVProjection(nn.Module):
     """model.py:76-126 with the hip producer.  The projection's q and k are
@@ -106,24 +119,35 @@ class QKVProjection(nn.Module):
         self.qkv_proj = nn.Linear(config.n_embd, self.q_dim + 2 * self.kv_dim, bias=False)
         self.rope = RotaryEmbedding(config.head_dim, config.rope_theta, config.rope_fraction)
 
-    def _project(self, x: torch.Tensor):
+    def _project(self, x: torch.Tensor, rotary: tuple[torch.Tensor, torch.Tensor] | None = None):
         bsz, seq_len, _ = x.shape
         q, k, v = self.qkv_proj(x).split((self.q_dim, self.kv_dim, self.kv_dim), dim=-1)
         q = q.view(bsz, seq_len, self.n_head, self.head_dim)
         k = k.view(bsz, seq_len, self.n_kv_head, self.head_dim)
         v = v.view(bsz, seq_len, self.n_kv_head, self.head_dim)
-        cos, sin = self.rope(seq_len, x.device, q.dtype)
+        cos, sin = self.rope(seq_len, x.device, q.dtype) if rotary is None else rotary
         return q, k, v, cos, sin
 
-    def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    def forward(
+        self, x: torch.Tensor, rotary: tuple[torch.Tensor, torch.Tensor] | None = None
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """rotary: the tokens' own (cos, sin) of RotaryEmbedding.at, for tokens
+        that continue a cache; None: positions 0 .. T - 1."""
         backend = normalize_module_backend("qkv_backend", self.config.qkv_backend)
         fwd_backend = getattr(self, f"fwd_{backend}", None)
         if fwd_backend is None:
             raise RuntimeError(f"{type(self).__name__} does not support backend {backend!r}")
-        return fwd_backend(x)
+        return fwd_backend(x) if rotary is None else fwd_backend(x, rotary)
 
-    def fwd_hip(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        q, k, v, cos, sin = self._project(x)
+    def fwd_hip(
+        self, x: torch.Tensor, rotary: tuple[torch.Tensor, torch.Tensor] | None = None
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        q, k, v, cos, sin = self._project(x, rotary)
+        if rotary is not None:  # the producer takes one table for its rows: all tokens as one sequence
+            tokens = q.shape[:2]
+            cos, sin = (t.reshape(-1, t.shape[-1]) for t in rotary)
+            q, k = kernels.qk_norm_rope_hip(q.flatten(0, 1)[None], k.flatten(0, 1)[None], cos, sin, self.config.norm_eps)
+            return q[0].unflatten(0, tokens), k[0].unflatten(0, tokens), v
         q, k = kernels.qk_norm_rope_hip(q, k, cos.transpose(1, 2), sin.transpose(1, 2), self.config.norm_eps)
         return q, k, v
 
@@ -176,6 +200,30 @@ class AttentionCore(nn.Module):
             attn_mask=None,
             window_size=self._attention_window_size(q.shape[1]),
             backend="hip",
+        )
+
+    def forward_cached(
+        self,
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        cache: KVCache,
+        starts: torch.Tensor | int,
+        counts: torch.Tensor | None = None,
+        prefix: KVCache | None = None,
+        prefix_length: int = 0,
+    ) -> torch.Tensor:
+        """Attention of new tokens of sequences whose earlier keys and values lie
+        in `cache`: stores the new k and v at starts .. and attends over the
+        layer's window of what is there, the new tokens among it (and over the
+        shared prefix before it).  The hip backend only; no backward.  Arguments
+        as in kernels.cached_attention_hip."""
+        backend = normalize_attention_backend(self.config.attention_backend)
+        if backend != "hip":
+            raise RuntimeError(f"{type(self).__name__} has no cached attention for backend {backend!r}")
+        kernels.kv_cache_write_hip(cache, k, v, starts, counts)
+        return kernels.cached_attention_hip(
+            q, cache, starts, counts, window_size=self.attention_window, prefix=prefix, prefix_length=prefix_length
         )
 
     def fwd_torch(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:

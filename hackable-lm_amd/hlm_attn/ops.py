@@ -695,13 +695,9 @@ hip_residual_rms_norm.register_autograd(_res_backward, setup_context=_res_setup_
 # --- the 8-bit key/value cache and attention over it ------------------------------
 #
 # hackable_lm::hip_kv_cache_write (mutates the cache), hip_kv_cache_read and
-# hip_cached_attn.  No backward: they serve generation and scoring.  Places are
-# an int (all sequences) or an int32 / int64 device tensor of one per sequence.
-
-
-def _no_grad_only(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"hip {what} has no backward: call it under torch.no_grad()")
+# hip_cached_attn.  No backward: they serve generation and scoring (kernels.py
+# refuses inputs that need a gradient).  Places are an int for all sequences
+# (`start`, with starts None) or an int32 / int64 device tensor.
 
 
 def _per_sequence(name: str, x: torch.Tensor | None, batch: int, device: torch.device) -> torch.Tensor | None:
@@ -725,11 +721,6 @@ def _cache_dims(name: str, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tens
                 and v_scale.shape == k_scale.shape and all(t.device == k.device and t.is_contiguous() for t in (k, v, k_scale, v_scale))):
             return B, Hkv, S, D
     raise RuntimeError(f"the {name} tensors are not those of a KVCache on one device")
-
-
-def _row_strides(t: torch.Tensor) -> ctypes.Array:
-    """strides3 for the cache's entry points, which look at no stride of a dim of one index."""
-    return _lib.strides3(t)
 
 
 def _cache_rows(name: str, t: torch.Tensor, device: torch.device, B: int, D: int) -> torch.Tensor:
@@ -762,7 +753,6 @@ def kv_cache_write_impl(
     if ext and cache_k.is_cuda:
         if ext.kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts, _raw_stream_of(cache_k.get_device())):
             return
-    _no_grad_only("kv_cache_write", k, v)
     B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
     k, v = _cache_rows("k", k, cache_k.device, B, D), _cache_rows("v", v, cache_k.device, B, D)
     if k.shape != v.shape or k.shape[2] != Hkv:
@@ -772,7 +762,7 @@ def kv_cache_write_impl(
     lib = _lib.load()
     with _on_device(k.device):
         rc = lib.hlm_attn_cache_write(
-            k.data_ptr(), v.data_ptr(), _row_strides(k), _row_strides(v), cache_k.data_ptr(), cache_v.data_ptr(),
+            k.data_ptr(), v.data_ptr(), _lib.strides3(k), _lib.strides3(v), cache_k.data_ptr(), cache_v.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), S, _ptr(starts), int(start), _ptr(counts),
             B, T, Hkv, D, _stream_handle(k.device),
         )
@@ -851,7 +841,6 @@ def cached_attn_impl(
                               prefix_v_scale, prefix_length, window, scale, _raw_stream_of(cache_k.get_device()))
         if res is not None:
             return res
-    _no_grad_only("cached_attention", q)
     B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
     q = _cache_rows("q", q, cache_k.device, B, D)
     T, H = q.shape[1], q.shape[2]
@@ -873,7 +862,7 @@ def cached_attn_impl(
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     with _on_device(q.device):
         rc = lib.hlm_attn_cached_fwd(
-            q.data_ptr(), _row_strides(q), o.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(),
+            q.data_ptr(), _lib.strides3(q), o.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), S, *places, _ptr(prefix_k), _ptr(prefix_v), _ptr(prefix_k_scale), _ptr(prefix_v_scale),
             prefix_slots, P, B, T, H, Hkv, D, int(window), float(scale), _ptr(ws), nbytes,
             _stream_handle(q.device),

@@ -312,3 +312,247 @@ def test_strided_queries_and_int64_places():
     assert not far.any()
     empty = hlm_attn.cached_attention_hip(q[:, :0], cache, starts)
     assert empty.shape == (2, 0, 4, 64)
+
+
+# --- a run of them together, graphs, streams, tracing --------------------------------------
+
+
+@pytest.mark.parametrize("layer,prefix_tokens", [(0, 0), (1, 0), (0, 70), (1, 70)])
+def test_a_generation_run_through_the_attention_core(layer, prefix_tokens):
+    """Prompts of different lengths in two chunks, drafted tokens, then single ones, in a local layer (window 96) and a full
+    one, with and without a shared context: each step against the oracle over the cache as it then is."""
+    g = torch.Generator().manual_seed(layer)
+    cfg = hlm_attn.AttentionConfig(n_layer=2, n_head=6, n_kv_head=2, attention_window=96, attention_full_every=2)
+    core = hlm_attn.AttentionCore(cfg, layer)
+    B, H, Hkv, D, S = 3, 6, 2, 64, 320
+    cache = hlm_attn.KVCache(B, S, Hkv, D)
+    plain = [(torch.zeros(B, Hkv, S, D, dtype=torch.long), torch.zeros(B, Hkv, S, dtype=torch.float64)) for _ in "kv"]
+    shared, prefix = (None, None)
+    if prefix_tokens:
+        shared, whole = filled(g, 1, prefix_tokens, Hkv, D)
+        prefix = [(c[:, :, :prefix_tokens], s[:, :, :prefix_tokens]) for c, s in whole]
+    lengths = [0, 0, 0]
+    for T, counts in ((130, [130, 57, 99]), (70, [20, 70, 0]), (4, [4, 4, 4]), (4, [1, 3, 4]), (1, [1, 1, 1]), (1, [1, 1, 1])):
+        q, k, v = _rand(g, B, T, H, D), _rand(g, B, T, Hkv, D), _rand(g, B, T, Hkv, D)
+        with torch.no_grad():
+            out = core.forward_cached(q.cuda(), k.cuda(), v.cuda(), cache, int32(lengths), int32(counts), shared, prefix_tokens)
+        for (c, s), x in zip(plain, (k, v)):
+            oracle.write(c, s, x, lengths, counts)
+        check_attention(out, q, *plain, lengths, counts, core.attention_window, prefix=prefix)
+        lengths = [n + m for n, m in zip(lengths, counts)]
+    for x, (c, s) in zip(hlm_attn.kv_cache_read_hip(cache, 0, S), plain):
+        assert torch.equal(x.cpu(), oracle.read(c, s, S, [0] * B, [S] * B).float().bfloat16())
+
+
+def test_a_cached_sequence_follows_the_uncached_attention():
+    """Token by token over the cache against attention() of the whole sequence: apart by the cache's rounding, half a step of
+    max|x| / 127 for each value and key (scores: 2^-8.9 of sum|q| max|k| scale at most)."""
+    g = torch.Generator().manual_seed(3)
+    B, T, H, Hkv, D, W = 2, 150, 4, 2, 64, 64
+    q, k, v = (_rand(g, B, T, h, D) for h in (H, Hkv, Hkv))
+    whole = hlm_attn.attention(q.cuda(), k.cuda(), v.cuda(), window_size=W).float()
+    cache = hlm_attn.KVCache(B, T, Hkv, D)
+    rows = []
+    for t in range(T):
+        hlm_attn.kv_cache_write_hip(cache, k[:, t : t + 1].cuda(), v[:, t : t + 1].cuda(), t)
+        rows.append(hlm_attn.cached_attention_hip(q[:, t : t + 1].cuda(), cache, t, window_size=W))
+    step = k.float().abs().amax() / 254
+    e = (q.float().abs().sum(-1).max() * step * D**-0.5).item()  # of a score
+    v_top = v.float().abs().max().item()
+    bound = v_top / 254 + v_top * 2 * (torch.tensor(e).exp().item() - 1) + 2**-7 * v_top
+    assert (torch.cat(rows, 1).float() - whole).abs().max().item() <= bound
+    assert ((torch.cat(rows, 1).float() - whole).norm() / whole.norm()).item() <= 0.03
+
+
+def test_a_step_is_captured_once_and_replayed_at_other_places():
+    """Write, attend and read back in one graph; starts, counts and the new tokens change between replays, with eager calls on
+    another cache and synchronisations in between."""
+    g = torch.Generator().manual_seed(11)
+    B, T, H, Hkv, D, S = 3, 2, 8, 2, 64, 1024
+    cache, plain = filled(g, B, S, Hkv, D)
+    other, other_plain = filled(g, B, S, Hkv, D)
+    shared, whole = filled(g, 1, 200, Hkv, D)
+    prefix = [(c[:, :, :200], s[:, :, :200]) for c, s in whole]
+    q, k, v = (torch.zeros(B, T, h, D, dtype=BF16, device="cuda") for h in (H, Hkv, Hkv))
+    starts, counts = int32([0] * B), int32([T] * B)
+
+    def step():
+        hlm_attn.kv_cache_write_hip(cache, k, v, starts, counts)
+        return (hlm_attn.cached_attention_hip(q, cache, starts, counts, 500),
+                hlm_attn.cached_attention_hip(q, cache, starts, counts, prefix=shared, prefix_length=200),
+                *hlm_attn.kv_cache_read_hip(cache, starts, T, counts))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    hlm_attn.kv_cache_write_hip(cache, torch.zeros(B, T, Hkv, D, dtype=BF16, device="cuda"), torch.zeros(B, T, Hkv, D, dtype=BF16, device="cuda"), starts)
+    for c, s in plain:
+        c[:, :, :T], s[:, :, :T] = 0, 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for places, n in (([0, 500, 1022], [2, 1, 2]), ([2, 501, 3], [2, 2, 0]), ([900, 64, 63], [1, 2, 2]), ([-1, 1023, 700], [2, 2, 2])):
+        new = [_rand(g, B, T, h, D) for h in (H, Hkv, Hkv)]
+        for to, x in zip((q, k, v), new):
+            to.copy_(x)
+        starts.copy_(int32(places)), counts.copy_(int32(n))
+        graph.replay()
+        for (c, s), x in zip(plain, new[1:]):
+            oracle.write(c, s, x, places, n)
+        eager = hlm_attn.cached_attention_hip(q, other, starts, counts)
+        check_attention(outs[0], new[0], *plain, places, n, 500)
+        check_attention(outs[1], new[0], *plain, places, n, prefix=prefix)
+        for x, (c, s) in zip(outs[2:], plain):
+            assert torch.equal(x.cpu(), oracle.read(c, s, T, places, n).float().bfloat16())
+        check_attention(eager, new[0], *other_plain, places, n)
+        torch.cuda.synchronize()
+
+
+def test_two_streams_over_one_cache():
+    """Calls that only read may overlap: each has its own workspace."""
+    g = torch.Generator().manual_seed(12)
+    cache, (k, v) = filled(g, 1, 4096, 4, 64)
+    qs = [_rand(g, 1, 1, 8, 64) for _ in range(2)]
+    on_gpu = [x.cuda() for x in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    outs = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(hlm_attn.cached_attention_hip(on_gpu[i], cache, 4095 - 64 * i))
+    torch.cuda.synchronize()
+    for i, x in enumerate(qs):
+        assert all(torch.equal(o, outs[i][0]) for o in outs[i])
+        check_attention(outs[i][0], x, k, v, [4095 - 64 * i], [1])
+
+
+@pytest.mark.parametrize("T", [1, 30])
+def test_results_do_not_change_from_call_to_call(T):
+    g = torch.Generator().manual_seed(13)
+    cache, _ = filled(g, 2, 2048, 4, 128)
+    shared, _ = filled(g, 1, 700, 4, 128)
+    q = _rand(g, 2, T, 12, 128).cuda()
+    first = hlm_attn.cached_attention_hip(q, cache, int32([1500, 77]), prefix=shared, prefix_length=700)
+    for _ in range(5):
+        assert torch.equal(first, hlm_attn.cached_attention_hip(q, cache, int32([1500, 77]), prefix=shared, prefix_length=700))
+
+
+def test_compiled_calls_run_the_kernels():
+    g = torch.Generator().manual_seed(14)
+    cache, plain = filled(g, 2, 128, 2, 64)
+    q, k, v = (_rand(g, 2, 3, h, 64) for h in (4, 2, 2))
+
+    def step(q, k, v, starts):
+        hlm_attn.kv_cache_write_hip(cache, k, v, starts)
+        return hlm_attn.cached_attention_hip(q * 2, cache, starts, window_size=50) + 1
+
+    with torch.no_grad():
+        out = torch.compile(step, fullgraph=True)(q.cuda(), k.cuda(), v.cuda(), int32([5, 100]))
+    for (c, s), x in zip(plain, (k, v)):
+        oracle.write(c, s, x, [5, 100], [3, 3])
+    eager = hlm_attn.cached_attention_hip((q * 2).cuda(), cache, int32([5, 100]), window_size=50)
+    assert torch.equal(out, eager + 1)
+    check_attention(eager, q * 2, *plain, [5, 100], [3, 3], 50)
+    for got, want in zip(plain_of(cache), plain):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_without_the_torch_extension(monkeypatch):
+    """The general path through the C ABI gives the same results, bit for bit."""
+    from hlm_attn import _lib
+
+    g = torch.Generator().manual_seed(15)
+    cache, _ = filled(g, 2, 256, 2, 64)
+    twin, _ = filled(torch.Generator().manual_seed(15), 2, 256, 2, 64)
+    shared, _ = filled(g, 1, 100, 2, 64)
+    q, k, v = (_rand(g, 2, 5, h, 64).cuda() for h in (4, 2, 2))
+    starts, counts = int32([100, 3]), int32([5, 4])
+
+    def run(c):
+        hlm_attn.kv_cache_write_hip(c, k, v, starts, counts)
+        return (hlm_attn.cached_attention_hip(q, c, starts, counts, 60), hlm_attn.cached_attention_hip(q, c, 20, prefix=shared, prefix_length=99),
+                *hlm_attn.kv_cache_read_hip(c, starts, 5, counts))
+
+    fast = run(cache)
+    monkeypatch.setattr(_lib, "_torch_fwd", False)
+    for a, b in zip(fast, run(twin)):
+        assert torch.equal(a, b)
+
+
+def test_refusals_on_the_device():
+    cache = hlm_attn.KVCache(2, 128, 2, 64)
+    x = torch.zeros(2, 3, 2, 64, dtype=BF16, device="cuda")
+    with pytest.raises(RuntimeError, match="do not fit"):
+        hlm_attn.kv_cache_write_hip(cache, x, x, 126)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        hlm_attn.cached_attention_hip(x, cache, -1)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        hlm_attn.kv_cache_read_hip(cache, 0, 129)
+    with pytest.raises(RuntimeError, match="starts"):
+        hlm_attn.kv_cache_write_hip(cache, x, x, torch.zeros(3, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="starts"):
+        hlm_attn.cached_attention_hip(x, cache, torch.zeros(2, dtype=torch.int32))  # on the CPU
+    with pytest.raises(RuntimeError, match="multiple of kv heads"):
+        hlm_attn.cached_attention_hip(torch.zeros(2, 1, 3, 64, dtype=BF16, device="cuda"), cache, 0)
+    with pytest.raises(RuntimeError, match="does not match a cache"):
+        hlm_attn.cached_attention_hip(x[:1], cache, 0)
+    with pytest.raises(RuntimeError, match="do not match"):
+        hlm_attn.kv_cache_write_hip(cache, x[:, :, :1], x[:, :, :1], 0)
+    with pytest.raises(RuntimeError, match="does not match"):
+        hlm_attn.cached_attention_hip(x, cache, 0, prefix=cache, prefix_length=5)  # two sequences
+    with pytest.raises(RuntimeError, match="scale"):
+        hlm_attn.cached_attention_hip(x, cache, 0, scale=-1.0)
+
+
+def test_a_cache_beyond_4_gib_of_keys():
+    """Byte offsets pass 2^31 and 2^32: all sequences of a cache of 5 GiB of keys, near their ends."""
+    g = torch.Generator().manual_seed(16)
+    B, Hkv, S, D, T, W = 5, 2, 1 << 22, 128, 80, 100
+    cache = hlm_attn.KVCache(B, S, Hkv, D)
+    assert cache.k.numel() > 4 << 30
+    starts = [S - 300, 5, S - 190, S - 250, S - 190]
+    k, v = _rand(g, B, 190, Hkv, D), _rand(g, B, 190, Hkv, D)
+    hlm_attn.kv_cache_write_hip(cache, k.cuda(), v.cuda(), int32(starts))
+    got = hlm_attn.kv_cache_read_hip(cache, int32(starts), 190)
+    plain = [oracle.encode(x) for x in (k, v)]
+    for x, (c, s) in zip(got, plain):
+        assert torch.equal(x.cpu(), (c.double() * s[..., None]).float().bfloat16())
+    for n in (1, T):  # the last n of those tokens
+        q = _rand(g, B, n, 4, D)
+        out = hlm_attn.cached_attention_hip(q.cuda(), cache, int32([s + 190 - n for s in starts]), window_size=W)
+        rows = [(c.transpose(1, 2), s.transpose(1, 2)) for c, s in plain]
+        check_attention(out, q, *rows, [190 - n] * B, [n] * B, W)
+
+
+def test_many_sequences_heads_and_rows():
+    """More workgroups than one wave of them, several tiles per unit, all variants of the prefix's and the own rows."""
+    g = torch.Generator().manual_seed(17)
+    for B, T, H, Hkv, D, P in ((20, 2, 8, 4, 64, 500), (5, 25, 6, 2, 64, 300), (3, 90, 4, 2, 64, 200), (9, 3, 4, 4, 128, 260), (2, 100, 6, 2, 128, 150)):
+        cache, (k, v) = filled(g, B, 192, Hkv, D)
+        shared, whole = filled(g, 1, P, Hkv, D)
+        q = _rand(g, B, T, H, D)
+        starts = [i * 7 % (192 - T) for i in range(B)]
+        out = hlm_attn.cached_attention_hip(q.cuda(), cache, int32(starts), prefix=shared, prefix_length=P)
+        check_attention(out, q, k, v, starts, [T] * B, prefix=[(c[:, :, :P], s[:, :, :P]) for c, s in whole])
+
+
+def test_the_producer_at_positions():
+    """QKVProjection with the tables of its tokens' positions: the rows that the producer gives those positions."""
+    cfg = hlm_attn.AttentionConfig(n_layer=1, n_head=4, n_kv_head=2, n_embd=64)
+    g = torch.Generator().manual_seed(18)
+    proj = hlm_attn.QKVProjection(cfg, 0)
+    with torch.no_grad():
+        proj.qkv_proj.weight.copy_(torch.randn(proj.qkv_proj.weight.shape, generator=g) * 0.1)
+        proj = proj.to("cuda", BF16)
+        proj.rope = hlm_attn.RotaryEmbedding(64).to("cuda")
+        x = _rand(g, 2, 5, 64).cuda()
+        pos = torch.tensor([[0, 1, 2, 3, 4], [40, 41, 42, 43, 44]], device="cuda")
+        q, k, v = proj(x, proj.rope.at(pos, BF16))
+        q0, k0, v0 = proj(x)
+        assert torch.equal(q[0], q0[0]) and torch.equal(k[0], k0[0]) and torch.equal(v, v0)
+        raw_q, raw_k, _, cos, sin = proj._project(x)
+        cos, sin = (t[0, 0] for t in proj.rope(50, x.device, BF16))
+        want = hlm_attn.qk_norm_rope_hip(raw_q[1:], raw_k[1:], cos[40:45].contiguous(), sin[40:45].contiguous(), cfg.norm_eps)
+        assert torch.equal(q[1:], want[0]) and torch.equal(k[1:], want[1])
