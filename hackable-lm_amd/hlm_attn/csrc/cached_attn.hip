@@ -759,7 +759,7 @@ hipError_t launch(const CachedAttnArgs& p, hipStream_t stream) {
 //    x (2 - x) of that, and takes 0.8 (head dim 64) or 1.4 for each round of its
 //    four waves.
 //  * Variants 1 and 2 take 1.0 or 1.15 for a block (1.15, 1.65 at head dim 128)
-//    while a CU has one or two workgroups, then 0.5 or 0.75 (0.8, 1.3) a
+//    while a CU has one or two workgroups, then 0.5 or 0.85 (0.8, 1.3) a
 //    workgroup: the larger tile costs less a row, the smaller spreads better.
 //  * Partial sums cost 3.0 for the second kernel (the prefix's are joined with
 //    the own ones in any case) and are written and read at 4.5 TB/s.
@@ -786,7 +786,7 @@ Split choose(int64_t rows, int64_t units, int64_t blocks, int64_t all_rows, bool
         t = std::max(rounds * (D == 64 ? 0.8 : 1.4), bytes / (4.8e6 * share * (2 - share)));
       } else {
         const double one = D == 64 ? (v == 1 ? 1.0 : 1.15) : (v == 1 ? 1.15 : 1.65);
-        const double more = D == 64 ? (v == 1 ? 0.5 : 0.75) : (v == 1 ? 0.8 : 1.3);
+        const double more = D == 64 ? (v == 1 ? 0.5 : 0.85) : (v == 1 ? 0.8 : 1.3);
         t = per * std::max(one, more * q);
       }
       if (n > 1 || joined) t += (joined ? 0.0 : 3.0) + n * (double)all_rows * row_us;
