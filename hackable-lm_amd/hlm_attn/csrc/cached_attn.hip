@@ -30,8 +30,8 @@
 // Numerics.  q is scaled by a power of two to at most 2 per row and then held
 // in fp16 (exact but for values 2^-14 of the row's largest and below, whose
 // error is 2^-25 of it); whole numbers are exact; products and sums are fp32.
-// p_j vs_j is rounded to fp16 relative to the largest vs so far, 2^11 at
-// p = 1: 11 bits for weights above 2^-25, and none above 2^-36 is lost.
+// p_j vs_j is rounded to fp16 relative to the largest vs that the row has seen
+// so far, 2^11 at p = 1: 11 bits for weights above 2^-25, and none above 2^-36 is lost.
 #include <cmath>
 #include <utility>
 
@@ -45,8 +45,8 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 constexpr float kWeightTop = 2048.f;  // a probability of 1 as fp16
 // The running maximum is moved only when a score passes it by 2^3, the value
-// scale that weights are relative to only when one passes it by 2: weights
-// reach 2^15, within fp16, and the sums stay where they are meanwhile.
+// scales that weights are relative to only when one passes the smallest by 2:
+// weights reach 2^15, within fp16, and the sums stay where they are meanwhile.
 constexpr float kSlack = 3.f;
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
@@ -69,13 +69,45 @@ __device__ __forceinline__ void each(F f) {
   each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-__device__ __forceinline__ float max_over_groups(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+// x op'ed over the 16 lanes of each group (DPP: the other of a pair, the other
+// pair of a quad, the mirrored quad of 8 lanes, the mirrored 8 of 16) and over
+// lane n of the four groups (the swaps of 16 and 32 lanes).  Both give every
+// lane the result, without LDS.
+template <int CTRL, class T>
+__device__ __forceinline__ T dpp(T x) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-__device__ __forceinline__ float sum_over_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+template <class T, class Op>
+__device__ __forceinline__ T over_lanes(T x, Op op) {
+  x = op(x, dpp<0xb1>(x));   // quad_perm 1 0 3 2
+  x = op(x, dpp<0x4e>(x));   // quad_perm 2 3 0 1
+  x = op(x, dpp<0x141>(x));  // row_half_mirror
+  return op(x, dpp<0x140>(x));  // row_mirror
+}
+template <class T, class Op>
+__device__ __forceinline__ T over_groups(T x, Op op) {
+  const unsigned a = __builtin_bit_cast(unsigned, x);
+  const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  x = op(__builtin_bit_cast(T, (unsigned)p[0]), __builtin_bit_cast(T, (unsigned)p[1]));
+  const unsigned b = __builtin_bit_cast(unsigned, x);
+  const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return op(__builtin_bit_cast(T, (unsigned)q[0]), __builtin_bit_cast(T, (unsigned)q[1]));
+}
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+};
+struct Min {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
+  __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); }
+};
+struct Sum {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+// A value that all lanes hold, as a scalar.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
 
 // Four codes (bytes c + 128) as fp16 whole numbers: 0x6400 | byte is 1024 + byte.
@@ -157,7 +189,10 @@ struct Rows {
   f16x8 q[NT][C][2];
   float rs[NT];             // scale log2(e) and q's power of two
   float mt[NT], l[NT];      // running maximum of (q.kc) ks, sum
-  float vtop, per_vtop;     // weights are relative to this value scale (0: none yet); its inverse
+  // The value scale that each row's weights are relative to: the largest that the
+  // row has seen (0: none yet), and its inverse.  The rows' smallest and largest,
+  // for the wave, and the largest's inverse: mostly they are the same.
+  float vtop[NT], per[NT], vlow, vhigh, per_vhigh;
   f32x4 o[NT][DT];          // o^T: dims 16 d + 4 g + i of row n
 
   // The rows r0 .. of a unit.  Queries are loaded before the places are known
@@ -192,17 +227,10 @@ struct Rows {
         inner_last = min(inner_last, hi[nt]);
       }
     }
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) {
-      first = min(first, __shfl_xor(first, m));
-      last = max(last, __shfl_xor(last, m));
-      inner_first = max(inner_first, __shfl_xor(inner_first, m));
-      inner_last = min(inner_last, __shfl_xor(inner_last, m));
-    }
-    first = __builtin_amdgcn_readfirstlane(first);
-    last = __builtin_amdgcn_readfirstlane(last);
-    inner_first = __builtin_amdgcn_readfirstlane(inner_first);
-    inner_last = __builtin_amdgcn_readfirstlane(inner_last);
+    first = uniform(over_lanes(first, Min()));
+    last = uniform(over_lanes(last, Max()));
+    inner_first = uniform(over_lanes(inner_first, Max()));
+    inner_last = uniform(over_lanes(inner_last, Min()));
   }
 
   __device__ __forceinline__ void take_q(const CachedAttnArgs& p, const bf16x8 x[NT][C][2]) {
@@ -218,8 +246,7 @@ struct Rows {
 #pragma unroll
           for (int e = 0; e < 8; ++e) top = max(top, (int)(bits[e] & 0x7fff));
         }
-      top = max(top, __shfl_xor(top, 16));
-      top = max(top, __shfl_xor(top, 32));
+      top = over_groups(top, Max());
       const int ex = min(126, max(-120, (top >> 7) - 127));
       const float down = __builtin_bit_cast(float, (127 - ex) << 23);
       // kept positive and finite: a score of -infinity times it stays what it is
@@ -231,11 +258,11 @@ struct Rows {
 #pragma unroll
           for (int e = 0; e < 8; ++e) q[nt][c][h][e] = (_Float16)((float)x[nt][c][h][e] * down);
       mt[nt] = -__builtin_inff();
-      l[nt] = 0.f;
+      l[nt] = vtop[nt] = per[nt] = 0.f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    vtop = per_vtop = 0.f;
+    vlow = vhigh = per_vhigh = 0.f;
   }
 
   // Scores sc of block k0 .. k0 + 63 (before the keys' scales; ks, vs: those of
@@ -258,27 +285,14 @@ struct Rows {
       }
       if (k0 + lane_key(lane) < first || k0 + lane_key(lane) > last) vs = 0.f;
     }
-    if (__any(vs > 2.f * vtop)) {
-      float top = vs;
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-      top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
-      const float f = vtop / top;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[nt][d] *= f;
-      vtop = top;
-      per_vtop = 1.f / top;  // <= 2^126: kWeightTop times it may be beyond fp32
-    }
-    vs = vs * per_vtop * kWeightTop;
+    if (__any(vs > 2.f * vlow)) raise_vtop(sc, vs);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = sc[nt][0][0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[nt][e / 4][e % 4]);
       if (__any((mx - mt[nt]) * rs[nt] > kSlack)) {
-        const float m = fmaxf(mt[nt], max_over_groups(mx));
+        const float m = fmaxf(mt[nt], over_groups(mx, Max()));
         const float alpha = m > mt[nt] ? __builtin_amdgcn_exp2f((mt[nt] - m) * rs[nt]) : 1.f;
         mt[nt] = m;
         l[nt] *= alpha;
@@ -295,22 +309,52 @@ struct Rows {
       }
       l[nt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    if (whole) {
+    if (whole && vlow == vhigh) {
+      const float rel = vs * per_vhigh * kWeightTop;  // 1 / vhigh <= 2^126: kWeightTop times it may be beyond fp32
       each<16>([&](auto e) {
-        const float f = row_lane<e>(vs);
+        const float f = row_lane<e>(rel);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) w[nt][e / 8][e % 8] = (_Float16)(sc[nt][e / 4][e % 4] * f);
       });
-    } else {
+    } else {  // a masked key's scale may be anything
       each<16>([&](auto e) {
         const float f = row_lane<e>(vs);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float pe = sc[nt][e / 4][e % 4];
-          w[nt][e / 8][e % 8] = (_Float16)(pe == 0.f ? 0.f : pe * f);
+          w[nt][e / 8][e % 8] = (_Float16)(pe == 0.f ? 0.f : f * per[nt] * kWeightTop * pe);
         }
       });
     }
+  }
+
+  // Raises the rows' value scales to those that they see in this block (rows that
+  // do not see a key, whose score is -infinity then, keep clear of its scale).
+  __device__ __forceinline__ void raise_vtop(const f32x4 sc[NT][4], float vs) {
+    float low = __builtin_inff(), high = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float top = 0.f;
+      each<16>([&](auto e) {
+        const float f = row_lane<e>(vs);
+        top = fmaxf(top, sc[nt][e / 4][e % 4] > -__builtin_inff() ? f : 0.f);
+      });
+      top = over_groups(top, Max());
+      if (top > vtop[nt]) {
+        const float f = vtop[nt] / top;
+        vtop[nt] = top;
+        per[nt] = 1.f / top;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[nt][d] *= f;
+      }
+      if (hi[nt] >= lo[nt]) {
+        low = fminf(low, vtop[nt]);
+        high = fmaxf(high, vtop[nt]);
+      }
+    }
+    vlow = uniform(over_lanes(low, Min()));
+    vhigh = uniform(over_lanes(high, Max()));
+    per_vhigh = vhigh > 0.f ? 1.f / vhigh : 0.f;
   }
 
   // The maximum in log2 units.
@@ -415,7 +459,7 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
   float* sums = lds + NW * ROWS * 2 + ROWS;                 // (NW, ROWS, LD)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const float l = sum_over_groups(rows.l[nt]);
+    const float l = over_groups(rows.l[nt], Sum());
     if (g == 0) {
       float* at = ml + (wave * ROWS + 16 * nt + n) * 2;
       at[0] = rows.top2(nt);
@@ -434,7 +478,7 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
     const float f = mine == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mine - m) / kWeightTop;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = rows.o[nt][d] * f * rows.vtop;
+      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = rows.o[nt][d] * f * rows.vtop[nt];
   }
   __syncthreads();
   constexpr int U = D / 4;
@@ -499,8 +543,8 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
     first = min(first, range[w]);
     last = max(last, range[4 + w]);
   }
-  first = __builtin_amdgcn_readfirstlane(first);
-  last = __builtin_amdgcn_readfirstlane(last);
+  first = uniform(first);
+  last = uniform(last);
   int begin, end;
   share(first, last, split, n_splits, begin, end);
   __syncthreads();  // range is read: the operands may overwrite it
@@ -591,7 +635,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
 
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const float l = sum_over_groups(rows.l[nt]);
+    const float l = over_groups(rows.l[nt], Sum());
     const int r = r0 + 16 * nt + n;
     if (r >= n_rows) continue;
     const int64_t out = row_of<PREFIX>(p, unit, r).out;
@@ -603,7 +647,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
         bf16x4 y = {};
         if (real)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = (bf16)(rows.o[nt][d][i] * f * rows.vtop);
+          for (int i = 0; i < 4; ++i) y[i] = (bf16)(rows.o[nt][d][i] * f * rows.vtop[nt]);
         *reinterpret_cast<bf16x4*>(p.o + out * D + 16 * d + 4 * g) = y;
       }
     } else {
@@ -615,7 +659,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
       }
       if (has)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * d + 4 * g) = rows.o[nt][d] / kWeightTop * rows.vtop;
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * d + 4 * g) = rows.o[nt][d] / kWeightTop * rows.vtop[nt];
     }
   }
 }

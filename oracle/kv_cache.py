@@ -47,7 +47,8 @@ def read(codes, scales, T: int, starts: list[int], counts: list[int]) -> torch.T
 
 
 def attention(q, k, v, starts, counts, window=None, scale=None, prefix=None):
-    """(o, a, s): the output (B, T, H, D); the sums of p |v|; the largest scale sum_d |q_d k_d| of each row.
+    """(o, a, s, v): the output (B, T, H, D); the sums of p |v|; of each row the largest scale sum_d |q_d k_d| and the largest
+    value scale that it sees.
 
     k and v are plain caches; prefix a pair of them of batch 1, cut to the prefix's length."""
     B, T, H, D = q.shape
@@ -55,7 +56,7 @@ def attention(q, k, v, starts, counts, window=None, scale=None, prefix=None):
     scale = D**-0.5 if scale is None else scale
     P = prefix[0][0].shape[2] if prefix else 0
     o, a = torch.zeros(B, T, H, D, dtype=torch.float64), torch.zeros(B, T, H, D, dtype=torch.float64)
-    reach = torch.zeros(B, T, H, dtype=torch.float64)
+    reach, top = torch.zeros(B, T, H, dtype=torch.float64), torch.zeros(B, T, H, dtype=torch.float64)
     for b, row in enumerate(positions(T, starts, counts, S)):
         for t, p in enumerate(row):
             if p < 0:
@@ -71,9 +72,11 @@ def attention(q, k, v, starts, counts, window=None, scale=None, prefix=None):
                         x = torch.cat((y, x))
                     rows.append(x)
                 kr, vr = rows
+                top[b, t, h] = max([v[1][b, g, max(0, first - P) : p + 1].nan_to_num().max().item()]
+                                   + ([prefix[1][1][0, g, min(first, P) :].nan_to_num().max().item()] if first < P else []))
                 qr = q[b, t, h].double()
                 prob = torch.softmax(kr @ qr * scale, dim=0)
                 o[b, t, h] = prob @ vr
                 a[b, t, h] = prob @ vr.abs()
                 reach[b, t, h] = (kr.abs() @ qr.abs()).max() * scale
-    return o, a, reach
+    return o, a, reach, top

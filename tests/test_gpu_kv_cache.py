@@ -7,7 +7,9 @@ Bounds, from the roundings made (eps / 2 of a type: bf16 2^-8, fp16 2^-11, fp32 
    scale sum_d |q_d k_d|; q in fp16 adds 2^-24 of the row's largest q per value, within (D + 4) 2^-24 of the same
    sum's bound with |q| at its largest, which the tests allow for by 2^-23 |q|max sum_d |k_d| scale.  A weight is off
    by 2 e_s + 2^-21 (exponential) + 2^-11 (fp16) relative, the normaliser by as much without the 2^-11, and sums of
-   n terms by n 2^-24; the output by 2^-8 relative for bf16.
+   n terms by n 2^-24; the output by 2^-8 relative for bf16.  Weights are held relative to the row's largest value scale vs,
+   2^11 at p = 1, so below fp16's normal range one is off by half its spacing there, 2^-25, that is by 2^-36 vs times a
+   whole number of at most 127 in the output: n 127 2^-36 vs in all (the sum of p is at least 1).
 """
 from __future__ import annotations
 
@@ -49,13 +51,13 @@ def int32(x):
 
 
 def check_attention(out, q, k, v, starts, counts, window=None, scale=None, prefix=None):
-    o, a, reach = oracle.attention(q, k, v, starts, counts, window, scale, prefix)
+    o, a, reach, top = oracle.attention(q, k, v, starts, counts, window, scale, prefix)
     D = q.shape[3]
     n = k[0].shape[2] + (prefix[0][0].shape[2] if prefix else 0)
     kmax = max((c[0].abs().sum(-1) * c[1]).nan_to_num().max().item() for c in ([k] + ([prefix[0]] if prefix else [])))
     e_s = (D + 4) * 2.0**-24 * reach + 2.0**-23 * q.double().abs().amax(-1) * kmax * (D**-0.5 if scale is None else scale)
     rel = 4 * e_s + 2.0**-20 + 2.0**-11 + n * 2.0**-23
-    tol = 2.0**-8 * o.abs() + a * rel[..., None] * (1 + 2.0**-8) + 1e-30
+    tol = 2.0**-8 * o.abs() + (a * rel[..., None] + (n * 127 * 2.0**-36 * top)[..., None]) * (1 + 2.0**-8) + 1e-30
     err = (out.double().cpu() - o).abs()
     assert out.dtype == BF16 and out.shape == q.shape
     assert torch.isfinite(out).all()
@@ -250,6 +252,24 @@ def test_scales_far_apart_and_one_key_that_takes_it_all(D):
     check_attention(out, big, kp, vp, [S - 5], [5], scale=1e-20)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,window", [(5, None), (5, 40), (60, None), (60, 30), (100, 50)])
+def test_rows_keep_clear_of_values_that_they_do_not_see(D, T, window):
+    """Values 2^80 above the others, behind some rows' positions and before others' windows, and after a prefix: rows that do
+    not see them lose nothing."""
+    g = torch.Generator().manual_seed(6)
+    S, start = 256, 120
+    v = _rand(g, 1, S, 2, D)
+    for at in (start + T // 2, start + T - 2, start - 25):
+        v[0, at] = (v[0, at].float() * 2.0**80).bfloat16()
+    cache, (kp, vp) = filled(g, 1, S, 2, D, None, v)
+    shared, whole = filled(g, 1, 150, 2, D)
+    q = _rand(g, 1, T, 4, D)
+    check_attention(hlm_attn.cached_attention_hip(q.cuda(), cache, start, None, window), q, kp, vp, [start], [T], window)
+    out = hlm_attn.cached_attention_hip(q.cuda(), cache, 0, None, window, prefix=shared, prefix_length=150)
+    check_attention(out, q, kp, vp, [0], [T], window, prefix=[(c[:, :, :150], s[:, :, :150]) for c, s in whole])
+
+
 @pytest.mark.parametrize("T", [1, 30, 70])
 def test_values_at_the_ends_of_the_range(T):
     g = torch.Generator().manual_seed(2)
@@ -260,7 +280,7 @@ def test_values_at_the_ends_of_the_range(T):
         cache, (kp, vp) = filled(g, 1, S, 1, D, None, v)
         q = _rand(g, 1, T, 2, D)
         out = hlm_attn.cached_attention_hip(q.cuda(), cache, S - T)
-        o, _, _ = oracle.attention(q, kp, vp, [S - T], [T])
+        o = oracle.attention(q, kp, vp, [S - T], [T])[0]
         # outputs below the smallest normal bf16 may come out as zeros
         assert ((out.double().cpu() - o).abs() <= 2.0**-6 * size + 2.0**-125).all()
         assert (out[..., 0].double().cpu() / size - 1).abs().max() <= 2.0**-7

@@ -67,7 +67,7 @@ def test_oracle_attention_is_the_dense_one():
     starts, counts = [0, 10, 30], [4, 2, 4]
     for window in (None, 1, 6, 100):
         for prefix in (None, [(codes[2], scales[2]), (codes[3], scales[3])]):
-            o, a, _ = oracle.attention(q, (codes[0], scales[0]), (codes[1], scales[1]), starts, counts, window, None, prefix)
+            o, a, _, top = oracle.attention(q, (codes[0], scales[0]), (codes[1], scales[1]), starts, counts, window, None, prefix)
             n = Pn if prefix else 0
             for b in range(B):
                 for t in range(T):
@@ -84,6 +84,8 @@ def test_oracle_attention_is_the_dense_one():
                         want = torch.softmax(s, 0) @ v
                         assert (o[b, t, h] - want).abs().max() <= 1e-12
                         assert (a[b, t, h] >= o[b, t, h].abs() - 1e-12).all()
+                        seen = torch.cat(([scales[3][0, h // 2]] if prefix else []) + [scales[1][b, h // 2]])[(lag >= 0) & (lag < (window or 10**6))]
+                        assert top[b, t, h] == seen.max()
 
 
 # --- the C ABI --------------------------------------------------------------------------
