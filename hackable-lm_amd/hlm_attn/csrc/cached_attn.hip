@@ -69,19 +69,11 @@ __device__ __forceinline__ void each(F f) {
   each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-// x op'ed over the 16 lanes of each group (DPP: the other of a pair, the other
-// pair of a quad, the mirrored quad of 8 lanes, the mirrored 8 of 16) and over
-// lane n of the four groups (the swaps of 16 and 32 lanes).  Both give every
-// lane the result, without LDS.
-template <int CTRL, class T>
-__device__ __forceinline__ T dpp(T x) {
-  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
+// x op'ed over the 16 lanes of each group, and over lane n of the four groups
+// (swaps of 16 and 32 lanes).  Both give every lane the result.
 template <class T, class Op>
 __device__ __forceinline__ T over_lanes(T x, Op op) {
-  x = op(x, dpp<0xb1>(x));   // quad_perm 1 0 3 2
-  x = op(x, dpp<0x4e>(x));   // quad_perm 2 3 0 1
-  x = op(x, dpp<0x141>(x));  // row_half_mirror
+  x = over_8_lanes(x, op);
   return op(x, dpp<0x140>(x));  // row_mirror
 }
 template <class T, class Op>
@@ -93,10 +85,6 @@ __device__ __forceinline__ T over_groups(T x, Op op) {
   const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
   return op(__builtin_bit_cast(T, (unsigned)q[0]), __builtin_bit_cast(T, (unsigned)q[1]));
 }
-struct Max {
-  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
-  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
-};
 struct Min {
   __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
   __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); }

@@ -42,6 +42,23 @@ __device__ __forceinline__ int64_t value_byte(int token, int d) {
 }
 constexpr float kCacheTiny = 1.504632769052528e-36f;  // 2^-119
 
+// x op'ed over 8 neighbouring lanes, for all of them, without LDS (DPP: the
+// other of a pair, the other pair of a quad, the mirrored quad).
+template <int CTRL, class T>
+__device__ __forceinline__ T dpp(T x) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <class T, class Op>
+__device__ __forceinline__ T over_8_lanes(T x, Op op) {
+  x = op(x, dpp<0xb1>(x));      // quad_perm 1 0 3 2
+  x = op(x, dpp<0x4e>(x));      // quad_perm 2 3 0 1
+  return op(x, dpp<0x141>(x));  // row_half_mirror
+}
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+};
+
 struct KvCache {
   uint8_t* k;
   uint8_t* v;

@@ -27,8 +27,8 @@ __device__ __forceinline__ void encode8(const bf16x8& x, unsigned u[8], float& s
   int top = 0;  // as bits, so that a NaN is the largest
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, (int)(bits[e] & 0x7fff));
-#pragma unroll
-  for (int m = D / 16; m >= 1; m >>= 1) top = max(top, __shfl_xor(top, m));
+  top = over_8_lanes(top, Max());
+  if constexpr (D == 128) top = max(top, dpp<0x140>(top));  // row_mirror
   const float a = __builtin_bit_cast(float, top << 16);
   const bool finite = top < 0x7f80, tiny = a < kCacheTiny;
   float r = tiny || !finite ? 0.f : 127.f / a;
