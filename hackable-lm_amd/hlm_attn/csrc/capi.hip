@@ -651,7 +651,10 @@ int run_cache_io(bool write, const void* k, const void* v, const int64_t* k_stri
   g_last_error[0] = '\0';
   if (B < 0 || T < 0 || Hkv <= 0) return fail(HLM_ATTN_EINVAL, "bad shape B=%d T=%d Hkv=%d", B, T, Hkv);
   if (D != 64 && D != 128) return fail(HLM_ATTN_EUNSUPPORTED, "head_dim %d is not supported (64 or 128)", D);
-  if ((int64_t)B * T >= ((int64_t)1 << 31) || (int64_t)B * T * Hkv >= ((int64_t)1 << 33))
+  // a launch has less than 2^32 threads: D / 8 for a row, or 4 D for a block of at most 64 tokens
+  const int64_t blocks = ((int64_t)T + 2 * hlm::kCacheBlock - 2) / hlm::kCacheBlock;
+  if ((int64_t)B * T >= ((int64_t)1 << 31) || (int64_t)B * T * Hkv >= ((int64_t)1 << 28) ||
+      (int64_t)B * Hkv * blocks * 4 * D >= ((int64_t)1 << 32))
     return fail(HLM_ATTN_EUNSUPPORTED, "too many rows for one launch");
   int rc = check_span(starts, start, counts, T, slots);
   if (rc) return rc;
@@ -691,8 +694,8 @@ int plan_cached(hlm::CachedAttnArgs& a, int64_t& ws_floats, int B, int T, int H,
                 hlm::kCacheBlock, kMaxSlots);
   if (prefix_length < 0 || prefix_length > kMaxSlots) return fail(HLM_ATTN_EINVAL, "bad prefix length %d", prefix_length);
   if (const int rc = check_span(starts, start, counts, T, slots)) return rc;
-  // rows are counted, and the partial sums' rows addressed, in ints
-  if ((int64_t)B * T > ((int64_t)1 << 30) || (int64_t)B * T * H > ((int64_t)1 << 30))
+  // rows are counted in ints, and a launch has less than 2^32 threads (up to 32 for a row)
+  if ((int64_t)B * T >= ((int64_t)1 << 27) || (int64_t)B * T * H >= ((int64_t)1 << 27))
     return fail(HLM_ATTN_EUNSUPPORTED, "too many query rows for one launch");
   ws_floats = 0;
   a.span = {starts, counts, start, T};
@@ -705,7 +708,7 @@ int plan_cached(hlm::CachedAttnArgs& a, int64_t& ws_floats, int B, int T, int H,
   if (B == 0 || T == 0) return HLM_ATTN_OK;
   const int64_t keys = starts == nullptr ? std::min<int64_t>(slots, (int64_t)start + T) : slots;
   const int64_t items = D == 64 ? hlm::plan_cached_attn<64>(a, keys) : hlm::plan_cached_attn<128>(a, keys);
-  if (items >= ((int64_t)1 << 31)) return fail(HLM_ATTN_EUNSUPPORTED, "problem too large for one launch");
+  if (items >= ((int64_t)1 << 24)) return fail(HLM_ATTN_EUNSUPPORTED, "too many query rows for one launch");
   const int splits = a.own_splits + a.prefix_splits;
   ws_floats = splits == 1 ? 0 : (int64_t)splits * B * T * H * (D + 2);
   return HLM_ATTN_OK;

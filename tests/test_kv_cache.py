@@ -101,7 +101,7 @@ def _write(lib, ptr=0x1000, slots=128, starts=None, start=0, counts=None, B=1, T
     return lib.hlm_attn_cache_write(p, p, s, s, p, p, p, p, slots, starts, start, counts, B, T, Hkv, D, None)
 
 
-def _read(lib, ptr=0x1000, slots=128, starts=None, start=0, counts=None, B=1, T=16, Hkv=2, D=64):
+def _read(lib, ptr=0x1000, slots=128, starts=None, start=0, counts=None, B=1, T=16, Hkv=2, D=64, strides=None):
     p = P(ptr) if ptr else None
     return lib.hlm_attn_cache_read(p, p, p, p, slots, p, p, starts, start, counts, B, T, Hkv, D, None)
 
@@ -120,6 +120,8 @@ CACHE_REFUSALS = [
     (dict(start=-1), -1, "do not fit"),
     (dict(start=129, counts=P(0x1000)), -1, "do not fit"),
     (dict(B=1 << 16, T=1 << 15), -2, "too many rows"),
+    (dict(B=1 << 14, T=1 << 13), -2, "too many rows"),  # 2^28 rows
+    (dict(B=1 << 21, T=16, Hkv=2, D=128, strides=(2048, 128, 128)), -2, "too many rows"),  # 2^23 blocks of 512 threads
 ]
 
 
@@ -127,7 +129,7 @@ CACHE_REFUSALS = [
 @pytest.mark.parametrize("call", [_write, _read])
 def test_cache_calls_reject_bad_arguments_before_touching_the_device(call, kwargs, code, msg):
     lib = _lib.load()
-    if kwargs.get("T", 0) > 128:
+    if "T" in kwargs:
         kwargs = dict(kwargs, starts=P(0x1000))
     assert call(lib, **kwargs) == code
     assert msg in lib.hlm_attn_last_error().decode()
@@ -170,6 +172,7 @@ def test_cached_attention_rejects_bad_arguments_before_touching_the_device():
         (dict(prefix_length=64, prefix_slots=64, prefix=P(0x1000), ws=0x1008), -1, "workspace"),
         (dict(prefix_length=64, prefix_slots=64, prefix=P(0x1000), ws_bytes=8), -1, "needed"),
         (dict(B=1 << 20, T=1 << 11, starts=P(0x1000)), -2, "too many query rows"),
+        (dict(B=1 << 24, T=1, H=4, Hkv=4, starts=P(0x1000)), -2, "too many query rows"),  # 2^26 workgroups
     ]:
         assert _attend(lib, **kwargs) == code, kwargs
         assert msg in lib.hlm_attn_last_error().decode(), (kwargs, lib.hlm_attn_last_error())
