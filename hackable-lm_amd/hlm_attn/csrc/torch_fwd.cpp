@@ -375,11 +375,11 @@ bool places_ready(const MaybeTensor& t, const at::Tensor& k, const CacheDims& c)
 const int32_t* places(const MaybeTensor& t) { return t ? t->data_ptr<int32_t>() : nullptr; }
 bool fits_int(int64_t x) { return x >= INT32_MIN && x <= INT32_MAX; }
 
-// Each returns false or nothing for inputs of the general path, which converts
-// or raises.
+// Each launches on the device's current stream, or returns false or nothing for
+// inputs of the general path, which converts or raises.
 bool kv_cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ck, const at::Tensor& cv,
                     const at::Tensor& ks, const at::Tensor& vs, const MaybeTensor& starts, int64_t start,
-                    const MaybeTensor& counts, int64_t stream) {
+                    const MaybeTensor& counts) {
   const CacheDims c = cache_dims(ck, cv, ks, vs);
   if (!cache_rows_ready(k, ck, c) || !cache_rows_ready(v, ck, c) || k.sizes() != v.sizes() || k.size(2) != c.Hkv ||
       !places_ready(starts, ck, c) || !places_ready(counts, ck, c) || !fits_int(start))
@@ -388,15 +388,14 @@ bool kv_cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
   const Strides sk(k), sv(v);
   check(hlm_attn_cache_write(k.data_ptr(), v.data_ptr(), sk.s, sv.s, ck.data_ptr(), cv.data_ptr(), ks.data_ptr<float>(),
                              vs.data_ptr<float>(), (int)c.slots, places(starts), (int)start, places(counts),
-                             (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3),
-                             reinterpret_cast<void*>(static_cast<uintptr_t>(stream))));
+                             (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3), stream_of(ck)));
   return true;
 }
 
 std::optional<std::tuple<at::Tensor, at::Tensor>> kv_cache_read(const at::Tensor& ck, const at::Tensor& cv,
                                                                 const at::Tensor& ks, const at::Tensor& vs,
                                                                 const MaybeTensor& starts, int64_t start,
-                                                                const MaybeTensor& counts, int64_t length, int64_t stream) {
+                                                                const MaybeTensor& counts, int64_t length) {
   const CacheDims c = cache_dims(ck, cv, ks, vs);
   if (c.slots == 0 || !places_ready(starts, ck, c) || !places_ready(counts, ck, c) || !fits_int(start) || length < 0 ||
       !fits_int(length))
@@ -406,14 +405,14 @@ std::optional<std::tuple<at::Tensor, at::Tensor>> kv_cache_read(const at::Tensor
   at::Tensor k = at::empty({c.B, length, c.Hkv, c.D}, options), v = at::empty({c.B, length, c.Hkv, c.D}, options);
   check(hlm_attn_cache_read(ck.data_ptr(), cv.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), (int)c.slots,
                             k.data_ptr(), v.data_ptr(), places(starts), (int)start, places(counts), (int)c.B, (int)length,
-                            (int)c.Hkv, (int)c.D, reinterpret_cast<void*>(static_cast<uintptr_t>(stream))));
+                            (int)c.Hkv, (int)c.D, stream_of(ck)));
   return std::make_tuple(k, v);
 }
 
 MaybeTensor cached_attn(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& ks,
                         const at::Tensor& vs, const MaybeTensor& starts, int64_t start, const MaybeTensor& counts,
                         const MaybeTensor& pk, const MaybeTensor& pv, const MaybeTensor& pks, const MaybeTensor& pvs,
-                        int64_t prefix_length, int64_t window, double scale, int64_t stream) {
+                        int64_t prefix_length, int64_t window, double scale) {
   const CacheDims c = cache_dims(ck, cv, ks, vs);
   if (!cache_rows_ready(q, ck, c) || !places_ready(starts, ck, c) || !places_ready(counts, ck, c) || !fits_int(start) ||
       !fits_int(window) || q.size(2) == 0 || q.size(2) % c.Hkv != 0)
@@ -439,8 +438,7 @@ MaybeTensor cached_attn(const at::Tensor& q, const at::Tensor& ck, const at::Ten
                             prefix ? pk->data_ptr() : nullptr, prefix ? pv->data_ptr() : nullptr,
                             prefix ? pks->data_ptr<float>() : nullptr, prefix ? pvs->data_ptr<float>() : nullptr,
                             (int)pc.slots, P, B, T, H, Hkv, D, (int)window, (float)scale,
-                            nbytes > 0 ? ws.data_ptr() : nullptr, nbytes,
-                            reinterpret_cast<void*>(static_cast<uintptr_t>(stream))));
+                            nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, stream_of(ck)));
   return o;
 }
 
@@ -454,10 +452,10 @@ PYBIND11_MODULE(_torch_fwd, m) {
   m.def("residual_rms_norm_train", &residual_rms_norm_train,
         "residual_rms_norm_train(residual, branch, eps) -> (out, normed), or None");
   m.def("kv_cache_write", &kv_cache_write,
-        "kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts, stream) -> whether it was done");
+        "kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts) -> whether it was done");
   m.def("kv_cache_read", &kv_cache_read,
-        "kv_cache_read(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length, stream) -> (k, v), or None");
+        "kv_cache_read(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length) -> (k, v), or None");
   m.def("cached_attn", &cached_attn,
         "cached_attn(q, cache_k, cache_v, k_scale, v_scale, starts, start, counts, prefix_k, prefix_v, prefix_k_scale, "
-        "prefix_v_scale, prefix_length, window, scale, stream) -> o, or None");
+        "prefix_v_scale, prefix_length, window, scale) -> o, or None");
 }

@@ -346,10 +346,6 @@ def residual_rms_norm_hip(residual: torch.Tensor, branch: torch.Tensor, eps: flo
 # for each new token (lm_eval_hackable_lm.py:185-207).
 
 
-def _places(starts: torch.Tensor | int) -> tuple[torch.Tensor | None, int]:
-    return (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
-
-
 def _head_padded(x: torch.Tensor, cache: "KVCache", name: str) -> torch.Tensor:
     """x as bf16 with the cache's kernel head dim, zero-padded where head_dim is none."""
     if x.requires_grad and torch.is_grad_enabled():
@@ -378,11 +374,16 @@ def kv_cache_write_hip(
     other than bf16 are rounded to it first.  No backward: tensors that require
     grad are refused outside torch.no_grad()."""
     ops = _ops or _load_ops()
+    first, start = (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+    direct = ops.direct_call_ok(k, v)
+    ext = ops.loaded_ext() if direct else None
+    if ext is not None and ext.kv_cache_write(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, first, start, counts):
+        return  # bf16 rows that the kernels read in place; all else is converted or refused below
     if v.shape != k.shape:
         raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
     k, v = _head_padded(k, cache, "k"), _head_padded(v, cache, "v")
-    run = ops.kv_cache_write_impl if ops.direct_call_ok(k, v) else ops.hip_kv_cache_write
-    run(k, v, *cache.tensors(), *_places(starts), counts)
+    run = ops.kv_cache_write_impl if direct else ops.hip_kv_cache_write
+    run(k, v, *cache.tensors(), first, start, counts)
 
 
 def kv_cache_read_hip(
@@ -392,9 +393,17 @@ def kv_cache_read_hip(
     (B, length, Hkv, D); starts and counts as in kv_cache_write_hip.  Padding
     and positions outside the cache, or never written, are zeros."""
     ops = _ops or _load_ops()
-    run = ops.kv_cache_read_impl if ops.direct_call_ok(cache.k) else ops.hip_kv_cache_read
-    k, v = run(*cache.tensors(), *_places(starts), counts, int(length))
-    return (k, v) if cache.kernel_dim == cache.head_dim else (k[..., : cache.head_dim], v[..., : cache.head_dim])
+    first, start = (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+    length = int(length)
+    direct = ops.direct_call_ok(cache.k)
+    ext = ops.loaded_ext() if direct else None
+    out = ext.kv_cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, first, start, counts, length) if ext is not None else None
+    if out is None:
+        run = ops.kv_cache_read_impl if direct else ops.hip_kv_cache_read
+        out = run(*cache.tensors(), first, start, counts, length)
+    if cache.kernel_dim != cache.head_dim:
+        out = (out[0][..., : cache.head_dim], out[1][..., : cache.head_dim])
+    return out
 
 
 def cached_attention_hip(
@@ -439,8 +448,15 @@ def cached_attention_hip(
         if not 0 <= prefix_length <= prefix.capacity:
             raise RuntimeError(f"prefix_length {prefix_length} is outside 0 .. {prefix.capacity}")
         shared = prefix.tensors()
-    q = _head_padded(q, cache, "q")
-    run = ops.cached_attn_impl if ops.direct_call_ok(q) else ops.hip_cached_attn
-    out = run(q, *cache.tensors(), *_places(starts), counts, *shared, int(prefix_length),
-              0 if window_size is None else int(window_size), float(scale))
+    window = 0 if window_size is None else int(window_size)
+    first, start = (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+    direct = ops.direct_call_ok(q)
+    ext = ops.loaded_ext() if direct else None
+    out = None
+    if ext is not None:
+        out = ext.cached_attn(q, cache.k, cache.v, cache.k_scale, cache.v_scale, first, start, counts, *shared, prefix_length, window, scale)
+    if out is None:
+        q = _head_padded(q, cache, "q")
+        run = ops.cached_attn_impl if direct else ops.hip_cached_attn
+        out = run(q, *cache.tensors(), first, start, counts, *shared, int(prefix_length), window, float(scale))
     return out if cache.kernel_dim == cache.head_dim else out[..., : cache.head_dim]

@@ -700,6 +700,12 @@ hip_residual_rms_norm.register_autograd(_res_backward, setup_context=_res_setup_
 # (`start`, with starts None) or an int32 / int64 device tensor.
 
 
+def loaded_ext():
+    """The torch extension, or None."""
+    ext = _lib._torch_fwd
+    return (_lib.torch_fwd() if ext is None else ext) or None
+
+
 def _per_sequence(name: str, x: torch.Tensor | None, batch: int, device: torch.device) -> torch.Tensor | None:
     """starts or counts as the kernels read them: int32 (batch,), contiguous."""
     if x is None:
@@ -744,15 +750,10 @@ def kv_cache_write_impl(
     k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scale: torch.Tensor,
     v_scale: torch.Tensor, starts: torch.Tensor | None, start: int, counts: torch.Tensor | None,
 ) -> None:
-    """The launch behind hackable_lm::hip_kv_cache_write.  Like its two
-    neighbours it runs as one call of the optional torch extension where the
-    inputs are as the kernels want them."""
-    ext = _lib._torch_fwd
-    if ext is None:
-        ext = _lib.torch_fwd()
-    if ext and cache_k.is_cuda:
-        if ext.kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts, _raw_stream_of(cache_k.get_device())):
-            return
+    """The launch behind hackable_lm::hip_kv_cache_write, through the C ABI with
+    any input that it can convert.  kernels.py tries the optional torch
+    extension first, as for its two neighbours: one C++ call that takes inputs
+    as the kernels want them."""
     B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
     k, v = _cache_rows("k", k, cache_k.device, B, D), _cache_rows("v", v, cache_k.device, B, D)
     if k.shape != v.shape or k.shape[2] != Hkv:
@@ -787,13 +788,6 @@ def kv_cache_read_impl(
     starts: torch.Tensor | None, start: int, counts: torch.Tensor | None, length: int,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The launch behind hackable_lm::hip_kv_cache_read."""
-    ext = _lib._torch_fwd
-    if ext is None:
-        ext = _lib.torch_fwd()
-    if ext and cache_k.is_cuda:
-        res = ext.kv_cache_read(cache_k, cache_v, k_scale, v_scale, starts, start, counts, length, _raw_stream_of(cache_k.get_device()))
-        if res is not None:
-            return res
     if cache_k.device.type != "cuda":
         raise RuntimeError(f"hip kv cache runs on ROCm devices only, got a cache on {cache_k.device}")
     B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
@@ -833,14 +827,6 @@ def cached_attn_impl(
     prefix_length: int, window: int, scale: float,
 ) -> torch.Tensor:
     """The launches behind hackable_lm::hip_cached_attn."""
-    ext = _lib._torch_fwd
-    if ext is None:
-        ext = _lib.torch_fwd()
-    if ext and cache_k.is_cuda:
-        res = ext.cached_attn(q, cache_k, cache_v, k_scale, v_scale, starts, start, counts, prefix_k, prefix_v, prefix_k_scale,
-                              prefix_v_scale, prefix_length, window, scale, _raw_stream_of(cache_k.get_device()))
-        if res is not None:
-            return res
     B, Hkv, S, D = _cache_dims("cache", cache_k, cache_v, k_scale, v_scale)
     q = _cache_rows("q", q, cache_k.device, B, D)
     T, H = q.shape[1], q.shape[2]

@@ -265,9 +265,9 @@ def test_tensors_that_are_no_cache_are_refused():
             ops._cache_dims("cache", *bad)
     ext = _lib.load_torch_fwd()
     x = torch.zeros(1, 1, 2, 64, dtype=BF16)
-    assert ext.kv_cache_write(x, x, k, v, ks, vs, None, 0, None, 0) is False  # CPU tensors: the general path's
-    assert ext.kv_cache_read(k, v, ks, vs, None, 0, None, 1, 0) is None
-    assert ext.cached_attn(x, k, v, ks, vs, None, 0, None, None, None, None, None, 0, 0, 0.125, 0) is None
+    assert ext.kv_cache_write(x, x, k, v, ks, vs, None, 0, None) is False  # CPU tensors: the general path's
+    assert ext.kv_cache_read(k, v, ks, vs, None, 0, None, 1) is None
+    assert ext.cached_attn(x, k, v, ks, vs, None, 0, None, None, None, None, None, 0, 0, 0.125) is None
 
 
 def test_fake_implementations_describe_shapes():
