@@ -645,9 +645,13 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
         p.part_ml[2 * at] = has ? rows.top2(nt) : -__builtin_inff();
         p.part_ml[2 * at + 1] = has ? l : 0.f;
       }
+      // past the caches' retention: 500 tokens over 1500 and 2500 27.6 -> 25.7 us
+      // (the few rows of attend_split: 16384 keys of 16 heads 18.3 -> 18.6, so not there)
       if (has)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * d + 4 * g) = rows.o[nt][d] / kWeightTop * rows.vtop[nt];
+        for (int d = 0; d < DT; ++d)
+          __builtin_nontemporal_store(rows.o[nt][d] / kWeightTop * rows.vtop[nt],
+                                      reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * d + 4 * g));
     }
   }
 }
