@@ -10,10 +10,21 @@
 // so the matrix products run on the whole numbers, which fp16 holds exactly,
 // and the scales multiply fp32 scores and probabilities.
 //
-// One workgroup takes 16 NT rows (the query heads of one kv head, of one or
-// more tokens; for the prefix, of all sequences) and a share of their keys in
-// blocks of 64; its four waves take the share's blocks in turn and their sums
-// are joined in LDS, those of several workgroups by the combine kernel.
+// A unit's rows are the query heads of one kv head, of one or more tokens; for
+// the prefix, of all sequences, so that its keys are read once.  Few rows
+// (attend_split): a workgroup takes 16 and a share of their keys in blocks of
+// 64, which its four waves take in turn; their sums are joined in LDS.  More
+// (attend_tile): 64 or 128 rows, shared out to the waves, and each block's
+// operands shared by them in LDS.  The sums of several workgroups over the same
+// rows' keys are joined by the combine kernel.
+//
+// Single tokens are bound by memory: 64 sequences of up to 2048 tokens, 12
+// heads of 64, 110.6 MB in 24.4 us (4.5 TB/s; a copy on this MI355X 4.8); 16384
+// keys of 16 heads of 128, 69 MB in 14.5 us and a join of 16 splits in 2 to 4.
+// Many rows are bound by the softmax's vector instructions, about 10 a score:
+// 2 x 500 tokens over 1500 and 2500, 12 heads of 64, 22.4 + 4.6 us.  A single
+// token over a window of 512 takes 5.3 us, most of it three trips to memory
+// (places, keys, rows of q with them) and the launch.
 //
 // Layouts (v_mfma_f32_16x16x32_f16, lane l, n = l % 16, g = l / 16):
 //   A (16 x 32): row n, k = 8 g + e;  B (32 x 16): k = 8 g + e, column n;

@@ -21,6 +21,9 @@ RMSNorm of each q and k row, then the partial rotary embedding.
 chunked linear + cross-entropy with the signature and result of
 kernels.py:945-959: the HIP cross-entropy rows in place of the Triton
 `linear_ce` op, inside this package's own chunk loop (`_LMHeadLoss`).
+
+`kv_cache_write_hip`, `kv_cache_read_hip` and `cached_attention_hip` store new
+tokens' keys and values in an 8-bit cache (cache.KVCache) and attend over it.
 """
 from __future__ import annotations
 
