@@ -349,6 +349,16 @@ def residual_rms_norm_hip(residual: torch.Tensor, branch: torch.Tensor, eps: flo
 # for each new token (lm_eval_hackable_lm.py:185-207).
 
 
+def _places(starts: torch.Tensor | int) -> tuple[torch.Tensor | None, int]:
+    """(a tensor of places, 0), or (None, the place of all sequences)."""
+    if isinstance(starts, torch.Tensor):
+        return starts, 0
+    start = int(starts)
+    if not -(2**31) <= start < 2**31:  # the C ABI's int would wrap
+        raise RuntimeError(f"starts {start} is no position of any cache")
+    return None, start
+
+
 def _head_padded(x: torch.Tensor, cache: "KVCache", name: str) -> torch.Tensor:
     """x as bf16 with the cache's kernel head dim, zero-padded where head_dim is none."""
     if x.requires_grad and torch.is_grad_enabled():
@@ -377,9 +387,9 @@ def kv_cache_write_hip(
     other than bf16 are rounded to it first.  No backward: tensors that require
     grad are refused outside torch.no_grad()."""
     ops = _ops or _load_ops()
-    first, start = (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+    first, start = _places(starts)
     direct = ops.direct_call_ok(k, v)
-    ext = ops.loaded_ext() if direct else None
+    ext = ops.loaded_ext() if direct and cache.kernel_dim == cache.head_dim else None
     if ext is not None and ext.kv_cache_write(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, first, start, counts):
         return  # bf16 rows that the kernels read in place; all else is converted or refused below
     if v.shape != k.shape:
@@ -396,7 +406,7 @@ def kv_cache_read_hip(
     (B, length, Hkv, D); starts and counts as in kv_cache_write_hip.  Padding
     and positions outside the cache, or never written, are zeros."""
     ops = _ops or _load_ops()
-    first, start = (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+    first, start = _places(starts)
     length = int(length)
     direct = ops.direct_call_ok(cache.k)
     ext = ops.loaded_ext() if direct else None
@@ -451,10 +461,10 @@ def cached_attention_hip(
         if not 0 <= prefix_length <= prefix.capacity:
             raise RuntimeError(f"prefix_length {prefix_length} is outside 0 .. {prefix.capacity}")
         shared = prefix.tensors()
-    window = 0 if window_size is None else int(window_size)
-    first, start = (starts, 0) if isinstance(starts, torch.Tensor) else (None, int(starts))
+    window = 0 if window_size is None else min(int(window_size), 2**31 - 1)
+    first, start = _places(starts)
     direct = ops.direct_call_ok(q)
-    ext = ops.loaded_ext() if direct else None
+    ext = ops.loaded_ext() if direct and cache.kernel_dim == cache.head_dim else None
     out = None
     if ext is not None:
         out = ext.cached_attn(q, cache.k, cache.v, cache.k_scale, cache.v_scale, first, start, counts, *shared, prefix_length, window, scale)

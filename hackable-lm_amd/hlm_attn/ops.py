@@ -739,7 +739,7 @@ def _cache_rows(name: str, t: torch.Tensor, device: torch.device, B: int, D: int
         raise RuntimeError(f"{name} {tuple(t.shape)} on {t.device} does not match a cache of {B} sequences with heads of {D} on {device}")
     s = t.stride()
     fits = s[3] == 1 and not t.data_ptr() & 15 and all(n <= 1 or (x >= 0 and not x & 7) for n, x in zip(t.shape[:3], s))
-    return t if fits else t.contiguous()
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
 def _ptr(t: torch.Tensor | None):

@@ -328,6 +328,11 @@ def test_strided_queries_and_int64_places():
     check_attention(out, q.cpu(), k, v, [20, 100], [3, 3])
     odd = _rand(g, 2, 3, 4, 65).cuda()[..., :64]  # no layout that the kernels read in place
     check_attention(hlm_attn.cached_attention_hip(odd, cache, starts), odd.cpu(), k, v, [20, 100], [3, 3])
+    flat = torch.zeros(2 * 3 * 4 * 64 + 4, dtype=BF16, device="cuda")
+    flat[4:] = q.flatten()
+    moved = flat[4:].view(2, 3, 4, 64)  # contiguous, but 8 bytes off
+    assert moved.data_ptr() % 16 == 8 and torch.equal(hlm_attn.cached_attention_hip(moved, cache, starts), out)
+    assert torch.equal(hlm_attn.cached_attention_hip(q, cache, starts, window_size=2**32 + 5), out)
     far = hlm_attn.cached_attention_hip(q, cache, torch.tensor([2**40, -(2**40)], device="cuda"))
     assert not far.any()
     empty = hlm_attn.cached_attention_hip(q[:, :0], cache, starts)
@@ -524,6 +529,10 @@ def test_refusals_on_the_device():
         hlm_attn.cached_attention_hip(x, cache, 0, prefix=cache, prefix_length=5)  # two sequences
     with pytest.raises(RuntimeError, match="scale"):
         hlm_attn.cached_attention_hip(x, cache, 0, scale=-1.0)
+    padded = hlm_attn.KVCache(2, 128, 2, 48)  # held in 64 dims, which is no head dim of its callers
+    for call in (lambda: hlm_attn.cached_attention_hip(x, padded, 0), lambda: hlm_attn.kv_cache_write_hip(padded, x, x, 0)):
+        with pytest.raises(RuntimeError, match="heads of 48"):
+            call()
 
 
 def test_a_cache_beyond_4_gib_of_keys():

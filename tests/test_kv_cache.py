@@ -243,6 +243,18 @@ def test_entry_points_refuse_cpu_tensors_gradients_and_mismatches():
         hlm_attn.cached_attention_hip(x, c, 0, prefix=hlm_attn.KVCache(1, 64, 2, 32, device="cpu"), prefix_length=5)
 
 
+def test_places_and_windows_beyond_32_bits():
+    """They would wrap in the C ABI's ints: refused, or held as the longest window there is."""
+    c = hlm_attn.KVCache(1, 64, 1, 64, device="cpu")
+    x = torch.zeros(1, 1, 1, 64, dtype=BF16)
+    for start in (2**32, 2**32 + 5, -(2**31) - 1, 2**31):
+        for call in (lambda: hlm_attn.kv_cache_write_hip(c, x, x, start), lambda: hlm_attn.kv_cache_read_hip(c, start, 1),
+                     lambda: hlm_attn.cached_attention_hip(x, c, start)):
+            with pytest.raises(RuntimeError, match="no position"):
+                call()
+    assert kernels._places(7) == (None, 7)
+
+
 def test_per_sequence_places_are_checked_and_converted():
     cpu = torch.device("cpu")
     assert ops._per_sequence("starts", None, 2, cpu) is None
