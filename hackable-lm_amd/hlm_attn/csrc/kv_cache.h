@@ -77,8 +77,8 @@ struct CacheSpan {
 
 // The position of token t of sequence b, or -1 for padding.
 __device__ __forceinline__ int64_t span_start(const CacheSpan& s, int b) { return s.starts ? s.starts[b] : s.start; }
-__device__ __forceinline__ int span_count(const CacheSpan& s, int b) {
-  return s.counts ? min(s.counts[b], s.T) : s.T;
+__device__ __forceinline__ int span_count(const CacheSpan& s, int b) {  // 0 .. T
+  return s.counts ? max(0, min(s.counts[b], s.T)) : s.T;
 }
 __device__ __forceinline__ int cache_position(int64_t start, int count, int t, int slots) {
   const int64_t p = start + t;

@@ -129,6 +129,20 @@ def test_rows_that_are_zero_tiny_huge_tied_or_not_finite():
     assert torch.isfinite(k[0, [0, 1, 2, 3, 4, 7, 8]]).all() and not k[0, [0, 1, 8]].any()
 
 
+@pytest.mark.parametrize("T", [3, 200])
+def test_negative_counts_are_none(T):
+    g = torch.Generator().manual_seed(T)
+    cache, plain = filled(g, 2, 256, 2, 64)
+    x = _rand(g, 2, T, 2, 64).cuda()
+    starts, counts = int32([5, 40]), torch.tensor([-(2**40), -1], device="cuda")
+    hlm_attn.kv_cache_write_hip(cache, x, x, starts, counts)
+    for (codes, scales), (want_c, want_s) in zip(plain_of(cache), plain):
+        assert torch.equal(codes, want_c) and torch.equal(scales, want_s)
+    for got in hlm_attn.kv_cache_read_hip(cache, starts, T, counts):
+        assert not got.any()
+    assert not hlm_attn.cached_attention_hip(_rand(g, 2, T, 4, 64).cuda(), cache, starts, counts).any()
+
+
 def test_unwritten_positions_read_as_zeros():
     cache = hlm_attn.KVCache(2, 100, 2, 64)
     assert cache.capacity == 128
