@@ -43,6 +43,8 @@
 // error is 2^-25 of it); whole numbers are exact; products and sums are fp32.
 // p_j vs_j is rounded to fp16 relative to the largest vs that the row has seen
 // so far, 2^11 at p = 1: 11 bits for weights above 2^-25, and none above 2^-36 is lost.
+// Neither sum can pass fp32 while keys are below 2^119 (q.k_j with q at 2, D = 128)
+// and values below 2^100 (2^24 keys at up to 2^3).
 #include <cmath>
 #include <utility>
 

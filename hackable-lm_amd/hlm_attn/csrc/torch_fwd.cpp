@@ -346,7 +346,7 @@ CacheDims cache_dims(const at::Tensor& k, const at::Tensor& v, const at::Tensor&
     return {};
   const int64_t B = ks.size(0), Hkv = ks.size(1), S = ks.size(2), pieces = k.size(3);
   const int64_t ksize[6] = {B, Hkv, S / 16, pieces, 16, 16}, vsize[7] = {B, Hkv, S / 64, pieces, 4, 16, 16};
-  if (S % 64 != 0 || S > INT32_MAX || k.sizes() != at::IntArrayRef(ksize, 6) || v.sizes() != at::IntArrayRef(vsize, 7) ||
+  if (Hkv == 0 || S % 64 != 0 || S > INT32_MAX || k.sizes() != at::IntArrayRef(ksize, 6) || v.sizes() != at::IntArrayRef(vsize, 7) ||
       vs.sizes() != ks.sizes())
     return {};
   if (!k.is_contiguous() || !v.is_contiguous() || !ks.is_contiguous() || !vs.is_contiguous() || v.device() != k.device() ||

@@ -28,6 +28,7 @@ tokens' keys and values in an 8-bit cache (cache.KVCache) and attend over it.
 from __future__ import annotations
 
 import math
+import operator
 from typing import TYPE_CHECKING, Any
 
 import torch
@@ -353,7 +354,7 @@ def _places(starts: torch.Tensor | int) -> tuple[torch.Tensor | None, int]:
     """(a tensor of places, 0), or (None, the place of all sequences)."""
     if isinstance(starts, torch.Tensor):
         return starts, 0
-    start = int(starts)
+    start = operator.index(starts)  # a float is no position
     if not -(2**31) <= start < 2**31:  # the C ABI's int would wrap
         raise RuntimeError(f"starts {start} is no position of any cache")
     return None, start
@@ -407,7 +408,7 @@ def kv_cache_read_hip(
     and positions outside the cache, or never written, are zeros."""
     ops = _ops or _load_ops()
     first, start = _places(starts)
-    length = int(length)
+    length = operator.index(length)
     direct = ops.direct_call_ok(cache.k)
     ext = ops.loaded_ext() if direct else None
     out = ext.kv_cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, first, start, counts, length) if ext is not None else None
@@ -445,7 +446,8 @@ def cached_attention_hip(
     ones behind them): its keys and values are read once for the whole batch.
     starts still counts own tokens, and the window reaches back into the prefix.
 
-    No backward: q that requires grad is refused outside torch.no_grad()."""
+    Keys up to 2^119 and values up to 2^100 leave room for every sum; beyond,
+    sums may overflow fp32.  No backward: q that requires grad is refused outside torch.no_grad()."""
     ops = _ops or _load_ops()
     if window_size is not None and window_size < 1:
         raise RuntimeError(f"window_size must be >= 1 or None, got {window_size}")

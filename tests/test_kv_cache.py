@@ -255,6 +255,15 @@ def test_places_and_windows_beyond_32_bits():
     assert kernels._places(7) == (None, 7)
 
 
+def test_places_that_are_no_whole_numbers_are_refused():
+    c = hlm_attn.KVCache(1, 64, 1, 64, device="cpu")
+    x = torch.zeros(1, 1, 1, 64, dtype=BF16)
+    for call in (lambda: hlm_attn.kv_cache_write_hip(c, x, x, 1.5), lambda: hlm_attn.kv_cache_read_hip(c, 0.0, 1),
+                 lambda: hlm_attn.kv_cache_read_hip(c, 0, 1.5), lambda: hlm_attn.cached_attention_hip(x, c, 2.0)):
+        with pytest.raises(TypeError):
+            call()
+
+
 def test_per_sequence_places_are_checked_and_converted():
     cpu = torch.device("cpu")
     assert ops._per_sequence("starts", None, 2, cpu) is None
