@@ -121,7 +121,7 @@ def build_torch_fwd() -> Path:
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_torch_fwd", "-DTORCH_API_INCLUDE_EXTENSION_H",
            *[f"-I{d}" for d in cpp_extension.include_paths()], f"-I{rocm / 'include'}", f"-I{sysconfig.get_paths()['include']}",
            str(CSRC / "torch_fwd.cpp"),
-           *[f"-L{d}" for d in cpp_extension.library_paths()], "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           *[f"-L{d}" for d in cpp_extension.library_paths()], "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
            f"-L{PKG_DIR}", "-lhlm_attn", "-Wl,-rpath,$ORIGIN"]
     tmp = TORCH_FWD_PATH.with_name(TORCH_FWD_PATH.name + ".tmp")
     _run([*cmd, "-o", str(tmp)])
