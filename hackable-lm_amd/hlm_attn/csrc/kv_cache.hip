@@ -201,12 +201,19 @@ __global__ __launch_bounds__(4 * D) void cache_write_blocks_kernel(CacheIoArgs p
   if (full || (token >= blk.lo && token < blk.hi)) *reinterpret_cast<u32x4*>(p.cache.k + base + byte) = kw;
   if (full) {
     *reinterpret_cast<u32x4*>(p.cache.v + base + byte) = vw;
-  } else {  // 16 bytes of values are tokens 16 t + 4 g + i, byte 4 t + i
+  } else {  // 16 bytes of values are tokens 16 t + 4 g + i, byte 4 t + i; four at a time where all are real
     const int g = byte / 256 % 4;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = 16 * (k / 4) + 4 * g + k % 4;
-      if (i >= blk.lo && i < blk.hi) p.cache.v[base + byte + k] = (uint8_t)(vw[k / 4] >> (8 * (k % 4)));
+    for (int t = 0; t < 4; ++t) {
+      const int i = 16 * t + 4 * g;
+      uint8_t* to = p.cache.v + base + byte + 4 * t;
+      if (i >= blk.lo && i + 4 <= blk.hi) {
+        *reinterpret_cast<unsigned*>(to) = vw[t];
+      } else {  // others' bytes are left alone, not rewritten: a call on another stream may own them
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k >= blk.lo && i + k < blk.hi) to[k] = (uint8_t)(vw[t] >> (8 * k));
+      }
     }
   }
 }
