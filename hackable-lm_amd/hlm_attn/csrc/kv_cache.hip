@@ -11,9 +11,10 @@
 //
 // Memory-bound: 4 D bytes in and 2 (D + 4) out per token and head to write, the
 // reverse to read.  On an MI355X: 8 sequences of 1024 to 2048 tokens, 12 heads of
-// 64, written in 16.1 us (4.0 TB/s), read in 13.8 (4.7 TB/s); 4 x 4096 tokens of
-// 12 heads of 128 read in 27.6 us (5.5 TB/s).  One token of 16 sequences: 4.2 and
-// 3.5 us, a launch and one trip to memory.
+// 64, written in 15.6 us (57.8 MB, 3.7 TB/s), read in 11.9 (70.4 MB with the
+// padding's zeros, 5.9 TB/s); 4 x 4096 tokens of 12 heads of 128 read in 24.0 us
+// (6.4 TB/s).  One token of 16 sequences: 4.0 and 3.4 us, a launch and one trip to
+// memory.
 #include "kv_cache.h"
 
 namespace hlm {
