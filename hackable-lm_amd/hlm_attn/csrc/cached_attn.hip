@@ -138,12 +138,17 @@ struct Row {
   int64_t out;
 };
 
-template <bool PREFIX>
+// The keys that a workgroup takes: a sequence's own, the prefix's for the rows of
+// all sequences, or the prefix's followed by the sequence's own (from the
+// prefix's next whole block on).
+enum Segment { kOwn, kPrefix, kBoth };
+
+template <Segment SEG>
 __device__ __forceinline__ Row row_of(const CachedAttnArgs& p, int unit, int r) {
   Row row;
   const int rt = fast_div(r, p.div_G), g = r - rt * p.G;
   int bt, h;
-  if constexpr (PREFIX) {
+  if constexpr (SEG == kPrefix) {
     bt = rt;
     row.b = fast_div(bt, p.div_T);
     row.t = bt - row.b * p.span.T;
@@ -159,20 +164,27 @@ __device__ __forceinline__ Row row_of(const CachedAttnArgs& p, int unit, int r) 
   return row;
 }
 
+// The first own key in kBoth's count of keys.
+__device__ __forceinline__ int own_key(const CachedAttnArgs& p) { return (p.P + kCacheBlock - 1) / kCacheBlock * kCacheBlock; }
+
 // The segment's keys lo .. hi that the row sees (hi < lo: none).
-template <bool PREFIX>
+template <Segment SEG>
 __device__ __forceinline__ void keys_seen(const CachedAttnArgs& p, const Row& row, int& lo, int& hi) {
   lo = 0;
   hi = -1;
   const int pos = cache_position(span_start(p.span, row.b), span_count(p.span, row.b), row.t, p.own.slots);
   if (pos < 0) return;
   const int64_t from = (int64_t)pos - p.window + 1;
-  if constexpr (PREFIX) {
+  const int in_prefix = (int)min((int64_t)p.P, max((int64_t)0, from + p.P)), in_own = (int)max((int64_t)0, from);
+  if constexpr (SEG == kPrefix) {
     hi = p.P - 1;
-    lo = (int)min((int64_t)p.P, max((int64_t)0, from + p.P));
-  } else {
+    lo = in_prefix;
+  } else if constexpr (SEG == kOwn) {
     hi = pos;
-    lo = (int)max((int64_t)0, from);
+    lo = in_own;
+  } else {
+    hi = own_key(p) + pos;
+    lo = in_prefix < p.P ? in_prefix : own_key(p) + in_own;
   }
 }
 
@@ -198,14 +210,14 @@ struct Rows {
 
   // The rows r0 .. of a unit.  Queries are loaded before the places are known
   // (of padding rows too, whose results nothing uses): both come from memory.
-  template <bool PREFIX>
+  template <Segment SEG>
   __device__ __forceinline__ void begin(const CachedAttnArgs& p, int unit, int r0, int n_rows, int lane, bf16x8 x[NT][C][2]) {
     const int n = lane & 15, g = lane >> 4;
     Row row[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + 16 * nt + n;
-      row[nt] = row_of<PREFIX>(p, unit, min(r, n_rows - 1));
+      row[nt] = row_of<SEG>(p, unit, min(r, n_rows - 1));
       const bf16* at = p.q + row[nt].b * p.sq[0] + row[nt].t * p.sq[1] + row[nt].head * p.sq[2] + 16 * g;
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -216,7 +228,7 @@ struct Rows {
     last = inner_first = -1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      keys_seen<PREFIX>(p, row[nt], lo[nt], hi[nt]);
+      keys_seen<SEG>(p, row[nt], lo[nt], hi[nt]);
       if (r0 + 16 * nt + n >= n_rows || hi[nt] < lo[nt]) {
         lo[nt] = 0;
         hi[nt] = -1;
@@ -267,10 +279,11 @@ struct Rows {
   }
 
   // Scores sc of block k0 .. k0 + 63 (before the keys' scales; ks, vs: those of
-  // key k0 + lane_key(lane)) into weights w, updating the rows' statistics.
-  __device__ __forceinline__ void weigh(f32x4 sc[NT][4], float ks, float vs, int k0, int lane, f16x8 w[NT][2]) {
+  // key k0 + lane_key(lane)) into weights w, updating the rows' statistics.  Keys
+  // of the block behind `end` are nobody's.
+  __device__ __forceinline__ void weigh(f32x4 sc[NT][4], float ks, float vs, int k0, int end, int lane, f16x8 w[NT][2]) {
     const int g = lane >> 4;
-    const bool whole = k0 >= inner_first && k0 + 63 <= inner_last;  // every row sees every key
+    const bool whole = k0 >= inner_first && k0 + 63 <= min(inner_last, end);  // every row sees every key
     each<16>([&](auto e) {
       const float f = row_lane<e>(ks);
 #pragma unroll
@@ -279,12 +292,12 @@ struct Rows {
     if (!whole) {  // selected, not added: masked slots may hold any scale
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const unsigned from = k0 + 4 * g - lo[nt], seen = max(0, hi[nt] - lo[nt] + 1);  // lo = 0 where hi < lo
+        const unsigned from = k0 + 4 * g - lo[nt], seen = max(0, min(hi[nt], end) - lo[nt] + 1);  // lo = 0 where hi < lo
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (from + (16 * (e / 4) + e % 4) >= seen) sc[nt][e / 4][e % 4] = -__builtin_inff();
       }
-      if (k0 + lane_key(lane) < first || k0 + lane_key(lane) > last) vs = 0.f;
+      if (k0 + lane_key(lane) < first || k0 + lane_key(lane) > min(last, end)) vs = 0.f;
     }
     if (__any(vs > 2.f * vlow)) raise_vtop(sc, vs);
 #pragma unroll
@@ -362,12 +375,33 @@ struct Rows {
   __device__ __forceinline__ float top2(int nt) const { return mt[nt] == -__builtin_inff() ? mt[nt] : mt[nt] * rs[nt]; }
 };
 
-// The head's rows of a cache.
-template <int D>
-__device__ __forceinline__ Keys keys_of(const KvCache& c, int unit) {
-  const int64_t head = (int64_t)unit * c.slots;
-  return {c.k + head * D, c.v + head * D, c.ks + head, c.vs + head};
-}
+// Where block blk of a unit's keys lies (keys: k, ks; values: v, vs), and the
+// last key that belongs to somebody as far as the block goes.
+template <int D, Segment SEG>
+struct Blocks {
+  Keys a, b;
+  int split, last;  // a's blocks are those before split, b's the others
+
+  static __device__ __forceinline__ Keys of(const KvCache& c, int unit) {
+    const int64_t head = (int64_t)unit * c.slots;
+    return {c.k + head * D, c.v + head * D, c.ks + head, c.vs + head};
+  }
+  __device__ __forceinline__ Blocks(const CachedAttnArgs& p, int unit) : split(own_key(p) / kCacheBlock), last(p.P - 1) {
+    if constexpr (SEG != kBoth) {
+      a = of(SEG == kPrefix ? p.prefix : p.own, unit);
+    } else {
+      a = of(p.prefix, unit % p.Hkv);
+      b = of(p.own, unit);
+    }
+  }
+  __device__ __forceinline__ Keys at(int blk) const {
+    const bool own = SEG == kBoth && blk >= split;
+    const Keys& s = own ? b : a;
+    const int n = own ? blk - split : blk;
+    return {s.k + (int64_t)n * (64 * D), s.v + (int64_t)n * (64 * D), s.ks + 64 * n, s.vs + 64 * n};
+  }
+  __device__ __forceinline__ int end(int blk) const { return SEG == kBoth && blk < split ? last : 0x7fffffff; }
+};
 
 // This workgroup's blocks begin .. end - 1 of the keys first .. last, shared
 // out evenly.
@@ -380,16 +414,16 @@ __device__ __forceinline__ void share(int first, int last, int split, int n_spli
 }
 
 // 16 NT rows, the keys shared by the four waves.
-template <int D, int NT, bool PREFIX>
+template <int D, int NT, Segment SEG>
 __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
                                              bool partial, float* lds) {
   constexpr int C = D / 64, DT = D / 16, ROWS = 16 * NT, LD = D + 4, NW = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int n_rows = PREFIX ? p.B * p.span.T * p.G : p.span.T * p.G;
-  const Keys s = keys_of<D>(PREFIX ? p.prefix : p.own, unit);
+  const int n_rows = SEG == kPrefix ? p.B * p.span.T * p.G : p.span.T * p.G;
+  const Blocks<D, SEG> keys(p, unit);
   Rows<D, NT> rows;
   bf16x8 x_q[NT][C][2];
-  rows.template begin<PREFIX>(p, unit, tile * ROWS, n_rows, lane, x_q);
+  rows.template begin<SEG>(p, unit, tile * ROWS, n_rows, lane, x_q);
   int begin, end;
   share(rows.first, rows.last, split, n_splits, begin, end);
 
@@ -398,16 +432,17 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
   u32x4 kr[4][C], vr[DT];
   float ksl = 0.f, vsl = 0.f;
   auto load_k = [&](int blk) {
-    const u32x4* at = reinterpret_cast<const u32x4*>(s.k + (int64_t)blk * (64 * D)) + lane;
-    ksl = s.ks[blk * 64 + lane_key(lane)];
-    vsl = s.vs[blk * 64 + lane_key(lane)];
+    const Keys s = keys.at(blk);
+    const u32x4* at = reinterpret_cast<const u32x4*>(s.k) + lane;
+    ksl = s.ks[lane_key(lane)];
+    vsl = s.vs[lane_key(lane)];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int c = 0; c < C; ++c) kr[t][c] = __builtin_nontemporal_load(at + (t * C + c) * 64);
   };
   auto load_v = [&](int blk) {
-    const u32x4* at = reinterpret_cast<const u32x4*>(s.v + (int64_t)blk * (64 * D)) + lane;
+    const u32x4* at = reinterpret_cast<const u32x4*>(keys.at(blk).v) + lane;
 #pragma unroll
     for (int d = 0; d < DT; ++d) vr[d] = __builtin_nontemporal_load(at + 64 * d);
   };
@@ -441,7 +476,7 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
       }
     }
     if (more) load_k(blk + NW);
-    rows.weigh(sc, ks, vs, blk * 64, lane, w);
+    rows.weigh(sc, ks, vs, blk * 64, keys.end(blk), lane, w);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f16x8 v0 = decode8(vr[d][0], vr[d][1]), v1 = decode8(vr[d][2], vr[d][3]);
@@ -486,7 +521,7 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
   for (int i = threadIdx.x; i < ROWS * U; i += 64 * NW) {
     const int rl = i / U, u = i % U, r = tile * ROWS + rl;
     if (r >= n_rows) continue;
-    const int64_t out = row_of<PREFIX>(p, unit, r).out;
+    const int64_t out = row_of<SEG>(p, unit, r).out;
     float m = ml[rl * 2];
 #pragma unroll
     for (int w = 1; w < NW; ++w) m = fmaxf(m, ml[(w * ROWS + rl) * 2]);
@@ -521,17 +556,17 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
 // 64 NT rows, 16 NT to a wave.  Each wave turns a quarter of a block's codes
 // into fp16 operands in LDS, in the order in which the lanes read them (1 KB to
 // an operand, one block ahead, no conflicts), and multiplies all of the block.
-template <int D, int NT, bool PREFIX>
+template <int D, int NT, Segment SEG>
 __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
                                             bool partial, float* lds) {
   constexpr int C = D / 64, DT = D / 16, VD = DT / 4, ROWS = 64 * NT, KF = 8 * C, F = KF + 2 * DT;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int n_rows = PREFIX ? p.B * p.span.T * p.G : p.span.T * p.G;
-  const Keys s = keys_of<D>(PREFIX ? p.prefix : p.own, unit);
+  const int n_rows = SEG == kPrefix ? p.B * p.span.T * p.G : p.span.T * p.G;
+  const Blocks<D, SEG> keys(p, unit);
   Rows<D, NT> rows;
   bf16x8 x_q[NT][C][2];
   const int r0 = tile * ROWS + wave * 16 * NT;
-  rows.template begin<PREFIX>(p, unit, r0, n_rows, lane, x_q);
+  rows.template begin<SEG>(p, unit, r0, n_rows, lane, x_q);
   int* range = reinterpret_cast<int*>(lds);
   if (lane == 0) {
     range[wave] = rows.first;
@@ -554,16 +589,18 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
   u32x4 kr[C], vr[VD];
   float ks_next = 0.f, vs_next = 0.f;
   auto load = [&](int blk) {
-    const u32x4* k = reinterpret_cast<const u32x4*>(s.k + (int64_t)blk * (64 * D)) + C * 64 * wave + lane;
-    const u32x4* v = reinterpret_cast<const u32x4*>(s.v + (int64_t)blk * (64 * D)) + VD * 64 * wave + lane;
+    const Keys s = keys.at(blk);
+    const u32x4* k = reinterpret_cast<const u32x4*>(s.k) + C * 64 * wave + lane;
+    const u32x4* v = reinterpret_cast<const u32x4*>(s.v) + VD * 64 * wave + lane;
 #pragma unroll
     for (int c = 0; c < C; ++c) kr[c] = k[64 * c];
 #pragma unroll
     for (int d = 0; d < VD; ++d) vr[d] = v[64 * d];
   };
   auto load_scales = [&](int blk) {
-    ks_next = s.ks[blk * 64 + lane_key(lane)];
-    vs_next = s.vs[blk * 64 + lane_key(lane)];
+    const Keys s = keys.at(blk);
+    ks_next = s.ks[lane_key(lane)];
+    vs_next = s.vs[lane_key(lane)];
   };
   auto store = [&](int buf) {
     f16x8* to = ops + buf * (F * 64) + lane;
@@ -621,7 +658,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
           for (int h = 0; h < 2; ++h) vf[d][h] = at[(KF + d * 2 + h) * 64];
         __builtin_amdgcn_sched_barrier(0);
       }
-      rows.weigh(sc, ks, vs, blk * 64, lane, w);
+      rows.weigh(sc, ks, vs, blk * 64, keys.end(blk), lane, w);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -639,7 +676,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
     const float l = over_groups(rows.l[nt], Sum());
     const int r = r0 + 16 * nt + n;
     if (r >= n_rows) continue;
-    const int64_t out = row_of<PREFIX>(p, unit, r).out;
+    const int64_t out = row_of<SEG>(p, unit, r).out;
     const bool real = rows.hi[nt] >= rows.lo[nt];
     if (!partial) {
       const float f = real ? 1.f / (l * kWeightTop) : 0.f;
@@ -677,17 +714,19 @@ constexpr int lds_floats(int variant) {
   return variant < 0 ? 0 : variant == 0 ? 16 * (1 + 4 * (2 + D + 4)) : 2 * (8 * (D / 64) + 2 * (D / 16)) * 64 * 4;
 }
 
-template <int D, int V, bool PREFIX>
+template <int D, int V, Segment SEG>
 __device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
                                        bool partial, float* lds) {
   if constexpr (V == 0)
-    attend_split<D, 1, PREFIX>(p, unit, tile, split, n_splits, slot, partial, lds);
+    attend_split<D, 1, SEG>(p, unit, tile, split, n_splits, slot, partial, lds);
   else
-    attend_tile<D, V, PREFIX>(p, unit, tile, split, n_splits, slot, partial, lds);
+    attend_tile<D, V, SEG>(p, unit, tile, split, n_splits, slot, partial, lds);
 }
 
 // Workgroups in order: the prefix's items (tile slowest), then the sequences'.
-// V, VP: variants of the own keys and of the prefix (-1: none).
+// V, VP: variants of the own keys and of the prefix (-1: none; kJoint: the
+// sequences' items take the prefix's keys as well).
+constexpr int kJoint = -2;
 template <int D, int V, int VP>
 __global__ __launch_bounds__(kThreads) void cached_attn_kernel(CachedAttnArgs p) {
   constexpr int own_lds = lds_floats<D>(V), prefix_lds = lds_floats<D>(VP);
@@ -697,14 +736,14 @@ __global__ __launch_bounds__(kThreads) void cached_attn_kernel(CachedAttnArgs p)
   if constexpr (VP >= 0) {
     if (id < p.prefix_items) {
       const int per = p.prefix_splits * p.Hkv, tile = id / per, rest = id - tile * per, split = rest / p.Hkv;
-      attend<D, VP, true>(p, rest - split * p.Hkv, tile, split, p.prefix_splits, split, partial, lds);
+      attend<D, VP, kPrefix>(p, rest - split * p.Hkv, tile, split, p.prefix_splits, split, partial, lds);
       return;
     }
     id -= p.prefix_items;
   }
   const int units = p.B * p.Hkv, st = id / units, unit = id - st * units;
   const int split = st / p.own_tiles, tile = st - split * p.own_tiles;
-  attend<D, V, false>(p, unit, p.own_tiles - 1 - tile, split, p.own_splits, p.prefix_splits + split, partial, lds);
+  attend<D, V, VP == kJoint ? kBoth : kOwn>(p, unit, p.own_tiles - 1 - tile, split, p.own_splits, p.prefix_splits + split, partial, lds);
 }
 
 // Joins the splits: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 4
@@ -815,12 +854,14 @@ hipError_t launch(const CachedAttnArgs& p, hipStream_t stream) {
 // `others` workgroups run beside these.
 struct Split {
   int variant, tiles, splits;
+  double us;
 };
+
+constexpr double kJoinUs = 3.0;
 
 template <int D>
 Split choose(int64_t rows, int64_t units, int64_t blocks, int64_t all_rows, bool joined, int64_t others) {
-  Split best{0, 1, 1};
-  double least = 1e300;
+  Split best{0, 1, 1, 1e300};
   const double row_us = (D + 2) * 8 / 4.5e6;
   for (int v = rows <= 16 ? 0 : 1; v <= (rows <= 16 ? 0 : rows <= 64 ? 1 : 2); ++v) {
     const int64_t tiles = (rows + tile_rows(v) - 1) / tile_rows(v), items = units * tiles;
@@ -838,11 +879,8 @@ Split choose(int64_t rows, int64_t units, int64_t blocks, int64_t all_rows, bool
         const double more = D == 64 ? (v == 1 ? 0.5 : 0.85) : (v == 1 ? 0.8 : 1.3);
         t = per * std::max(one, more * q);
       }
-      if (n > 1 || joined) t += (joined ? 0.0 : 3.0) + n * (double)all_rows * row_us;
-      if (t < 0.97 * least) {  // a later choice needs to be clearly better
-        least = t;
-        best = {v, (int)tiles, n};
-      }
+      if (n > 1 || joined) t += (joined ? 0.0 : kJoinUs) + n * (double)all_rows * row_us;
+      if (t < 0.97 * best.us) best = {v, (int)tiles, n, t};  // a later choice needs to be clearly better
     }
   }
   return best;
@@ -856,10 +894,7 @@ template <int D>
 int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys) {
   const int64_t rows = (int64_t)p.span.T * p.G, units = (int64_t)p.B * p.Hkv, all = (int64_t)p.B * p.span.T * p.H;
   const int64_t reach = std::min(keys, (int64_t)p.window + p.span.T + 64);
-  const Split own = choose<D>(rows, units, (reach + 63) / 64, all, p.P > 0, 0);
-  p.variant = own.variant;
-  p.own_tiles = own.tiles;
-  p.own_splits = own.splits;
+  Split own = choose<D>(rows, units, (reach + 63) / 64, all, p.P > 0, 0);
   p.prefix_variant = -1;
   p.prefix_tiles = p.prefix_splits = 0;
   if (p.P > 0) {
@@ -867,10 +902,26 @@ int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys) {
     Split pre = choose<D>(rows * p.B, p.Hkv, (seen + 63) / 64 + 1, all, true, units * own.tiles * own.splits);
     // one kernel for both: 128-row tiles of a sequence's rows need them of the prefix's
     if (pre.variant < own.variant) pre.variant = own.variant, pre.tiles = (int)((rows * p.B + 127) / 128);
-    p.prefix_variant = pre.variant;
-    p.prefix_tiles = pre.tiles;
-    p.prefix_splits = pre.splits;
+    // Or each sequence's rows over both: the prefix is read once per sequence, mostly
+    // from the caches, but there is no join, or a smaller one.  Few rows go there at
+    // par, tiles up to where the model has it 15% above, from some 200 measured shapes:
+    // 24 x 1 token over a prefix of 60, 6 heads of 64, 5.9 against 8.3 us (over 800,
+    // 10.3 and 9.4); 32 x 64 tokens over 50, 12 heads of 64 in 4 groups, 10.1 and 15.8
+    // (over 1500, 34.3 and 34.1); 4 x 37 over 1000 in a window of 512, 10.4 and 11.5.
+    const int64_t total = std::min(keys + p.P + 63, (int64_t)p.window + p.span.T + 64 + 63);
+    const Split both = choose<D>(rows, units, (total + 63) / 64, all, false, 0);
+    if (both.us < (both.variant > 0 ? 1.15 : 1.0) * (std::max(own.us, pre.us) + kJoinUs)) {
+      own = both;
+      p.prefix_variant = kJoint;
+    } else {
+      p.prefix_variant = pre.variant;
+      p.prefix_tiles = pre.tiles;
+      p.prefix_splits = pre.splits;
+    }
   }
+  p.variant = own.variant;
+  p.own_tiles = own.tiles;
+  p.own_splits = own.splits;
   const int64_t prefix_items = (int64_t)p.Hkv * p.prefix_tiles * p.prefix_splits;
   p.prefix_items = (int)prefix_items;
   return prefix_items + units * p.own_tiles * p.own_splits;
@@ -878,6 +929,10 @@ int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys) {
 
 template <int D>
 hipError_t launch_cached_attn(const CachedAttnArgs& p, hipStream_t stream) {
+  if (p.prefix_variant == kJoint) {
+    if (p.variant == 0) return launch<D, 0, kJoint>(p, stream);
+    return p.variant == 1 ? launch<D, 1, kJoint>(p, stream) : launch<D, 2, kJoint>(p, stream);
+  }
   switch (4 * p.variant + p.prefix_variant) {
     case 4 * 0 - 1: return launch<D, 0, -1>(p, stream);
     case 4 * 1 - 1: return launch<D, 1, -1>(p, stream);

@@ -214,6 +214,40 @@ def test_attention_with_a_shared_prefix(B, T, H, Hkv, D, capacity, starts, count
     check_attention(out, q, k, v, starts, [T] * B if counts is None else counts, window, prefix=prefix)
 
 
+JOINT = [
+    # B, T, H, Hkv, starts, counts, window, P
+    (1, 1, 2, 2, [0], None, None, 1),
+    (5, 1, 6, 2, [0, 63, 64, 100, 190], None, None, 63),
+    (5, 2, 6, 2, [0, 63, 64, 100, 190], [2, 1, 0, 2, 2], None, 64),
+    (3, 3, 4, 4, [-1, 60, 189], None, None, 65),
+    (3, 1, 4, 4, [3, 60, 150], None, 61, 100),  # windows that end in the prefix, at the first own key, behind it
+    (3, 1, 4, 4, [59, 60, 61], None, 61, 100),
+    (2, 40, 4, 2, [0, 90], [40, 17], None, 70),
+    (2, 40, 4, 2, [0, 90], [40, 17], 50, 70),
+    (8, 64, 3, 1, [0, 10, 20, 30, 40, 50, 60, 70], None, None, 50),
+    (8, 150, 2, 2, [0] * 8, [150, 149, 1, 0, 64, 65, 128, 150], 30, 100),
+    (8, 150, 2, 2, [0] * 8, [150, 149, 1, 0, 64, 65, 128, 150], None, 100),
+    (32, 65, 16, 16, list(range(32)), None, None, 70),  # tiles of 128 rows
+    (32, 65, 16, 16, list(range(32)), [65, 1] * 16, 80, 70),
+]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,T,H,Hkv,starts,counts,window,P", JOINT)
+def test_a_short_prefix_and_the_own_keys_in_one_pass(B, T, H, Hkv, starts, counts, window, P, D):
+    """The prefix's last block ends in slots that belong to nobody, whatever these hold."""
+    g = torch.Generator().manual_seed(B * T + P)
+    cache, (k, v) = filled(g, B, 192, Hkv, D)
+    shared, whole = filled(g, 1, 192, Hkv, D)
+    for scale, fill in ((shared.k_scale, float("nan")), (shared.v_scale, float("inf"))):
+        scale[:, :, P:] = fill
+    q = _rand(g, B, T, H, D, scale=1.5)
+    n = [T] * B if counts is None else counts
+    out = hlm_attn.cached_attention_hip(q.cuda(), cache, int32(starts), None if counts is None else int32(counts), window,
+                                        prefix=shared, prefix_length=P)
+    check_attention(out, q, k, v, starts, n, window, prefix=[(c[:, :, :P], s[:, :, :P]) for c, s in whole])
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T,window", [(1, None), (1, 70), (40, None), (40, 33)])
 def test_masked_slots_may_hold_anything(D, T, window):

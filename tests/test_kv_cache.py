@@ -168,9 +168,9 @@ def test_cached_attention_rejects_bad_arguments_before_touching_the_device():
         (dict(prefix_length=10), -1, "multiple of 64"),
         (dict(prefix_length=10, prefix_slots=64), -1, "prefix tensor is null"),
         (dict(prefix_length=65, prefix_slots=64, prefix=P(0x1000)), -1, "beyond its 64 slots"),
-        (dict(prefix_length=64, prefix_slots=64, prefix=P(0x1000), ws=None), -1, "workspace"),
-        (dict(prefix_length=64, prefix_slots=64, prefix=P(0x1000), ws=0x1008), -1, "workspace"),
-        (dict(prefix_length=64, prefix_slots=64, prefix=P(0x1000), ws_bytes=8), -1, "needed"),
+        (dict(prefix_length=8192, prefix_slots=8192, prefix=P(0x1000), ws=None), -1, "workspace"),
+        (dict(prefix_length=8192, prefix_slots=8192, prefix=P(0x1000), ws=0x1008), -1, "workspace"),
+        (dict(prefix_length=8192, prefix_slots=8192, prefix=P(0x1000), ws_bytes=8), -1, "needed"),
         (dict(B=1 << 20, T=1 << 11, starts=P(0x1000)), -2, "too many query rows"),
         (dict(B=1 << 24, T=1, H=4, Hkv=4, starts=P(0x1000)), -2, "too many query rows"),  # 2^26 workgroups
     ]:
@@ -194,10 +194,12 @@ def test_workspace_is_a_whole_number_of_partial_outputs_and_bounded(D):
                             row = B * T * H * (D + 2) * 4
                             assert n >= 0 and n % row == 0
                             assert n // row <= (128 if prefix else 64)
-                            assert prefix == 0 or n >= 2 * row
     assert fn(1, 1, 12, 12, D, 1 << 17, some, 0, None, 0, 64) == 0  # a short window needs no splits
     assert fn(1, 1, 4, 4, D, 1 << 17, None, 63, None, 0, 0) == 0  # nor does a short cache that the host knows of
     assert fn(1, 1, 4, 4, D, 1 << 17, some, 0, None, 0, 0) > 0
+    assert fn(1, 1, 4, 4, D, 64, some, 0, None, 60, 0) == 0  # a short prefix is taken with the own keys
+    for prefix, window, n in ((8000, 0, 2), (60, 0, 0)):  # many samples: a long one once for all of them
+        assert fn(64, 1, 12, 12, D, 64, some, 0, None, prefix, window) >= n * 64 * 12 * (D + 2) * 4
     assert fn(1, 0, 4, 4, D, 64, some, 0, None, 0, 0) == 0 and fn(1, 1, 4, 4, 96, 64, some, 0, None, 0, 0) == -2
 
 
