@@ -11,7 +11,8 @@
 // and the scales multiply fp32 scores and probabilities.
 //
 // A unit's rows are the query heads of one kv head, of one or more tokens; for
-// the prefix, of all sequences, so that its keys are read once.  Few rows
+// the prefix, of all sequences, so that its keys are read once (a short one's
+// are taken by each sequence together with its own: plan_cached_attn).  Few rows
 // (attend_split): a workgroup takes 16 and a share of their keys in blocks of
 // 64, which its four waves take in turn; their sums are joined in LDS.  More
 // (attend_tile): 64 or 128 rows, shared out to the waves, and each block's

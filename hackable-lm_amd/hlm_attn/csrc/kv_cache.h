@@ -108,7 +108,7 @@ struct CachedAttnArgs {
   int window;  // >= 1
   float scale_log2;
   FastDiv div_G, div_T;
-  int variant, prefix_variant;  // of the kernel, by its rows (-1: no prefix)
+  int variant, prefix_variant;  // of the kernel, by its rows (-1: no prefix, -2: with the own keys)
   // Splits of the keys: own_splits workgroups share a sequence's keys (for one
   // tile of its rows), prefix_splits the prefix's.
   int own_splits, prefix_splits, own_tiles, prefix_tiles, prefix_items;
