@@ -152,19 +152,12 @@ def _inputs(case, seed):
     return s
 
 
-_package = None
-
-
 def _hlm():
-    """The framework's package, imported once as a user's program does."""
-    global _package
-    if _package is None:
-        if os.path.abspath("hackable-lm_amd") not in sys.path:
-            sys.path.insert(0, os.path.abspath("hackable-lm_amd"))
-        import hlm_attn
+    if os.path.abspath("hackable-lm_amd") not in sys.path:
+        sys.path.insert(0, os.path.abspath("hackable-lm_amd"))
+    import hlm_attn
 
-        _package = hlm_attn
-    return _package
+    return hlm_attn
 
 
 def _cache_of(k, v, capacity):
