@@ -23,6 +23,7 @@ import os
 
 import torch
 from torch.autograd import forward_ad
+from torch.utils._device import DeviceContext
 from torch.utils.flop_counter import register_flop_formula
 
 from . import _lib
@@ -98,13 +99,26 @@ def _on_index(index: int):
     return torch.cuda.device(index)
 
 
+def _ops_watched() -> bool:
+    """Whether something active has to see the custom ops themselves: tracing,
+    a dispatch mode, a function transform, forward-mode AD."""
+    return (torch.compiler.is_compiling() or bool(torch._C._len_torch_dispatch_stack())
+            or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._get_tracing_state() is not None
+            or forward_ad._current_level >= 0)
+
+
 def direct_call_ok(*tensors: torch.Tensor) -> bool:
     """True when a call may skip torch's op dispatcher and run the kernels'
-    Python implementation directly: plain tensors (not fake or traced), no
-    torch.compile tracing in progress, and no input that needs a gradient
-    (inference, e.g. the evaluation harness's no-grad forwards).  The
-    dispatcher and autograd wrapper cost far more host time than the launch."""
-    if torch.compiler.is_compiling():
+    Python implementation directly: plain tensors (not fake or traced), nothing
+    active that has to see the op (function modes among them, but for a default
+    device, which changes no tensor that the calls make), and no input that
+    needs a gradient (inference, e.g. the evaluation harness's no-grad
+    forwards).  The dispatcher and autograd wrapper cost far more host time than
+    the launch."""
+    if _ops_watched():
+        return False
+    if torch._C._len_torch_function_stack() and not all(
+            type(m) is DeviceContext for m in torch.overrides._get_current_function_mode_stack()):
         return False
     grad = torch.is_grad_enabled()
     for t in tensors:
@@ -118,9 +132,7 @@ def eager_ext(*tensors: torch.Tensor):
     C++ autograd functions instead of the custom op, else None: plain tensors
     and parameters, and nothing active that has to see the op itself (tracing,
     a dispatch or function mode, a function transform, forward-mode AD)."""
-    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack()
-            or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._get_tracing_state() is not None
-            or forward_ad._current_level >= 0):
+    if _ops_watched() or torch._C._len_torch_function_stack():
         return None
     for t in tensors:
         if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:

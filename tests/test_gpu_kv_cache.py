@@ -633,3 +633,45 @@ def test_the_producer_at_positions():
         cos, sin = (t[0, 0] for t in proj.rope(50, x.device, BF16))
         want = hlm_attn.qk_norm_rope_hip(raw_q[1:], raw_k[1:], cos[40:45].contiguous(), sin[40:45].contiguous(), cfg.norm_eps)
         assert torch.equal(q[1:], want[0]) and torch.equal(k[1:], want[1])
+
+
+# --- calls that something watches -------------------------------------------------------------
+
+
+def test_traced_calls_hold_the_write_and_run_again():
+    """make_fx and jit.trace record the write and the attention; the recorded step run on other tokens does both."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    B, T, H, Hkv, D, S = 2, 3, 4, 2, 64, 128
+    for trace in (lambda f, a: make_fx(f)(*a), lambda f, a: torch.jit.trace(f, a, check_trace=False)):
+        g = torch.Generator().manual_seed(21)
+        cache, plain = filled(g, B, S, Hkv, D)
+
+        def step(q, k, v, starts):
+            hlm_attn.kv_cache_write_hip(cache, k, v, starts)
+            return hlm_attn.cached_attention_hip(q, cache, starts, window_size=50)
+
+        with torch.no_grad():
+            first = [_rand(g, B, T, h, D) for h in (H, Hkv, Hkv)]
+            recorded = trace(step, (*(x.cuda() for x in first), int32([5, 60])))
+            for (c, s), x in zip(plain, first[1:]):  # tracing ran the step
+                oracle.write(c, s, x, [5, 60], [T, T])
+            q, k, v = (_rand(g, B, T, h, D) for h in (H, Hkv, Hkv))
+            out = recorded(q.cuda(), k.cuda(), v.cuda(), int32([100, 20]))
+        for (c, s), x in zip(plain, (k, v)):
+            oracle.write(c, s, x, [100, 20], [T, T])
+        for got, want in zip(plain_of(cache), plain):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        check_attention(out, q, *plain, [100, 20], [T, T], 50)
+
+
+def test_attention_over_vmap_is_that_of_its_parts():
+    g = torch.Generator().manual_seed(22)
+    cache, plain = filled(g, 2, 128, 2, 64)
+    q = _rand(g, 3, 2, 1, 4, 64)
+    with torch.no_grad():
+        out = torch.func.vmap(lambda x: hlm_attn.cached_attention_hip(x, cache, 100))(q.cuda())
+        for a, b in zip(out, q):
+            assert torch.equal(a, hlm_attn.cached_attention_hip(b.cuda(), cache, 100))
+        with pytest.raises(RuntimeError, match="[Bb]atching rule"):
+            torch.func.vmap(lambda x: (hlm_attn.kv_cache_write_hip(cache, x, x, 0), x)[1])(_rand(g, 3, 2, 1, 2, 64).cuda())

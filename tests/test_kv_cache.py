@@ -329,3 +329,69 @@ def test_attention_core_caches_on_the_hip_backend_only(monkeypatch):
     core.config.attention_backend = "torch"
     with pytest.raises(RuntimeError, match="no cached attention"):
         core.forward_cached("q", "k", "v", "cache", 0)
+
+
+# --- calls that something watches -------------------------------------------------------------
+
+
+class _Seen(torch.utils._python_dispatch.TorchDispatchMode):
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+class _Functions(torch.overrides.TorchFunctionMode):
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+def _watched(f):
+    """f(x) under each thing that has to see the ops themselves."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.zeros(2, 3, 2, 64, dtype=BF16)
+    with _Seen():
+        f(x)
+    with _Functions():
+        f(x)
+    with forward_ad.dual_level():
+        f(x)
+    make_fx(lambda x: (f(x), x + 1)[1])(x)
+    torch.jit.trace(lambda x: (f(x), x + 1)[1], (x,), check_trace=False)
+    torch.func.vmap(lambda x: (f(x), x)[1])(x[None])
+    torch.func.functionalize(lambda x: (f(x), x + 1)[1])(x)
+
+
+def test_direct_calls_stand_aside_where_the_op_must_be_seen():
+    x = torch.zeros(2, 3, 2, 64, dtype=BF16)
+    taken = []
+    with torch.no_grad():
+        _watched(lambda x: taken.append(ops.direct_call_ok(x, x)))
+        assert taken == [False] * 7
+        with torch.device("cpu"):  # a default device is a function mode that changes nothing for them
+            assert ops.direct_call_ok(x)
+        assert ops.direct_call_ok(x)
+
+
+def test_cache_calls_reach_their_ops_where_something_watches(monkeypatch):
+    """A traced write that launches at once would be missing from the trace, and the attention's output a constant in it."""
+    c = hlm_attn.KVCache(2, 64, 2, 64, device="cpu")
+    seen, direct = [], []
+    for name in ("write", "read", "attn"):
+        op, impl = (f"hip_kv_cache_{name}", f"kv_cache_{name}_impl") if name != "attn" else ("hip_cached_attn", "cached_attn_impl")
+        monkeypatch.setattr(ops, op, lambda *a, name=name: seen.append(name))
+        monkeypatch.setattr(ops, impl, lambda *a, name=name: direct.append(name))
+    monkeypatch.setattr(ops, "hip_attn_fwd", lambda *a: (seen.append("attention"), None))
+    monkeypatch.setattr(ops, "attn_fwd_impl", lambda *a: (direct.append("attention"), None))
+
+    def step(x):
+        hlm_attn.kv_cache_write_hip(c, x, x, 0)
+        hlm_attn.cached_attention_hip(x, c, 0)
+        hlm_attn.kv_cache_read_hip(c, 0, 3)
+        hlm_attn.attention(x, x, x)
+
+    with torch.no_grad():
+        _watched(step)
+        assert seen == ["write", "attn", "read", "attention"] * 7 and not direct
+        step(torch.zeros(2, 3, 2, 64, dtype=BF16))
+        assert direct == ["write", "attn", "read", "attention"]
