@@ -7,6 +7,8 @@ KVCache's fields; read values back with kv_cache_read_hip.
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from .kernels import padded_head_dim
@@ -33,12 +35,13 @@ class KVCache:
     """
 
     def __init__(self, batch: int, capacity: int, n_kv_head: int, head_dim: int, device: torch.device | str = "cuda") -> None:
+        batch, capacity, n_kv_head, head_dim = map(operator.index, (batch, capacity, n_kv_head, head_dim))
         for name, n in (("batch", batch), ("capacity", capacity), ("n_kv_head", n_kv_head)):
             if n < 1:
                 raise RuntimeError(f"{name} must be at least 1, got {n}")
-        self.batch, self.n_kv_head, self.head_dim = int(batch), int(n_kv_head), int(head_dim)
+        self.batch, self.n_kv_head, self.head_dim = batch, n_kv_head, head_dim
         self.kernel_dim = padded_head_dim(head_dim, head_dim)
-        self.capacity = -(-int(capacity) // BLOCK) * BLOCK
+        self.capacity = -(-capacity // BLOCK) * BLOCK
         if self.capacity > 1 << 24:
             raise RuntimeError(f"capacity {capacity} is beyond {1 << 24} tokens")
         shape = (self.batch, self.n_kv_head, self.capacity)

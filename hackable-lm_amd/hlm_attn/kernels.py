@@ -450,8 +450,11 @@ def cached_attention_hip(
     Keys up to 2^119 and values up to 2^100 leave room for every sum; beyond,
     sums may overflow fp32.  No backward: q that requires grad is refused outside torch.no_grad()."""
     ops = _ops or _load_ops()
-    if window_size is not None and window_size < 1:
-        raise RuntimeError(f"window_size must be >= 1 or None, got {window_size}")
+    if window_size is not None:
+        window_size = operator.index(window_size)  # half a token is no window
+        if window_size < 1:
+            raise RuntimeError(f"window_size must be >= 1 or None, got {window_size}")
+    prefix_length = operator.index(prefix_length)
     if scale is None:
         scale = 1.0 / math.sqrt(cache.head_dim)
     if prefix is None:
@@ -464,7 +467,7 @@ def cached_attention_hip(
         if not 0 <= prefix_length <= prefix.capacity:
             raise RuntimeError(f"prefix_length {prefix_length} is outside 0 .. {prefix.capacity}")
         shared = prefix.tensors()
-    window = 0 if window_size is None else min(int(window_size), 2**31 - 1)
+    window = 0 if window_size is None else min(window_size, 2**31 - 1)
     first, start = _places(starts)
     direct = ops.direct_call_ok(q)
     ext = ops.loaded_ext() if direct and cache.kernel_dim == cache.head_dim else None
@@ -474,5 +477,5 @@ def cached_attention_hip(
     if out is None:
         q = _head_padded(q, cache, "q")
         run = ops.cached_attn_impl if direct else ops.hip_cached_attn
-        out = run(q, *cache.tensors(), first, start, counts, *shared, int(prefix_length), window, float(scale))
+        out = run(q, *cache.tensors(), first, start, counts, *shared, prefix_length, window, float(scale))
     return out if cache.kernel_dim == cache.head_dim else out[..., : cache.head_dim]

@@ -395,3 +395,40 @@ def test_cache_calls_reach_their_ops_where_something_watches(monkeypatch):
         assert seen == ["write", "attn", "read", "attention"] * 7 and not direct
         step(torch.zeros(2, 3, 2, 64, dtype=BF16))
         assert direct == ["write", "attn", "read", "attention"]
+
+
+# --- sizes --------------------------------------------------------------------------------
+
+
+def test_sizes_that_are_no_whole_numbers_are_refused():
+    """A window of 512.5 is none: it was cut to 512."""
+    import numpy as np
+
+    c = hlm_attn.KVCache(2, 64, 2, 64, device="cpu")
+    x = torch.zeros(2, 3, 2, 64, dtype=BF16)
+    one = hlm_attn.KVCache(1, 64, 2, 64, device="cpu")
+    for call in (lambda: hlm_attn.cached_attention_hip(x, c, 0, window_size=512.5), lambda: hlm_attn.cached_attention_hip(x, c, 0, window_size=20.0),
+                 lambda: hlm_attn.cached_attention_hip(x, c, 0, prefix=one, prefix_length=3.5),
+                 lambda: hlm_attn.KVCache(1.5, 64, 2, 64, device="meta"), lambda: hlm_attn.KVCache(1, 100.5, 2, 64, device="meta"),
+                 lambda: hlm_attn.KVCache(1, 64, 2.0, 64, device="meta"), lambda: hlm_attn.KVCache(1, 64, 2, 64.0, device="meta")):
+        with pytest.raises(TypeError):
+            call()
+    whole = hlm_attn.KVCache(np.int64(1), np.int64(100), np.int32(2), np.int16(80), device="cpu")
+    assert (whole.batch, whole.capacity, whole.n_kv_head, whole.head_dim) == (1, 128, 2, 80)
+    with pytest.raises(RuntimeError, match="ROCm devices only"):  # whole numbers of any type pass
+        hlm_attn.cached_attention_hip(x, c, np.int64(0), window_size=np.int64(20), prefix=one, prefix_length=np.int32(3))
+
+
+def test_compiled_calls_take_whole_numbers_that_vary():
+    """torch.compile traces the checks, as constants and as sizes that change: on the CPU the call ends at the op itself."""
+    c = hlm_attn.KVCache(2, 64, 2, 64, device="cpu")
+    one = hlm_attn.KVCache(1, 64, 2, 64, device="cpu")
+    x = torch.zeros(2, 3, 2, 64, dtype=BF16)
+
+    def attend(x, start, window, n):
+        return hlm_attn.cached_attention_hip(x, c, start, window_size=window, prefix=one, prefix_length=n)
+
+    run = torch.compile(attend, fullgraph=True, backend="eager")
+    for start, window, n in ((0, 5, 7), (1, 6, 8), (2, 9, 10)):
+        with pytest.raises(RuntimeError, match="ROCm devices only"), torch.no_grad():
+            run(x, start, window, n)
