@@ -694,8 +694,9 @@ int plan_cached(hlm::CachedAttnArgs& a, int64_t& ws_floats, int B, int T, int H,
                 hlm::kCacheBlock, kMaxSlots);
   if (prefix_length < 0 || prefix_length > kMaxSlots) return fail(HLM_ATTN_EINVAL, "bad prefix length %d", prefix_length);
   if (const int rc = check_span(starts, start, counts, T, slots)) return rc;
-  // rows are counted in ints, and a launch has less than 2^32 threads (up to 32 for a row)
-  if ((int64_t)B * T >= ((int64_t)1 << 27) || (int64_t)B * T * H >= ((int64_t)1 << 27))
+  // rows are counted in ints, and a launch has less than 2^32 threads (up to 32 for
+  // a row, 8 rows to a workgroup of the join)
+  if ((int64_t)B * T >= ((int64_t)1 << 27) || (int64_t)B * T * H > ((int64_t)1 << 27) - 8)
     return fail(HLM_ATTN_EUNSUPPORTED, "too many query rows for one launch");
   ws_floats = 0;
   a.span = {starts, counts, start, T};

@@ -358,7 +358,7 @@ int hlm_attn_cache_read(const void* cache_k, const void* cache_v, const float* k
  * null) all sequences see the prefix at positions 0 .. prefix_length - 1 and
  * their own tokens behind it, at prefix_length + starts[b] + t.
  *   q  bf16 (B, T, H, D), strides as k's above;  o  bf16 (B, T, H, D), contiguous
- * H % Hkv == 0; scale > 0; B T H < 2^27.  ws (16-byte aligned, no
+ * H % Hkv == 0; scale > 0; B T H <= 2^27 - 8.  ws (16-byte aligned, no
  * initialisation needed, not shared by calls that may overlap) holds
  * hlm_attn_cached_fwd_workspace_bytes bytes for the same sizes and places.
  * Nothing is allocated and the host never waits.

@@ -432,3 +432,15 @@ def test_compiled_calls_take_whole_numbers_that_vary():
     for start, window, n in ((0, 5, 7), (1, 6, 8), (2, 9, 10)):
         with pytest.raises(RuntimeError, match="ROCm devices only"), torch.no_grad():
             run(x, start, window, n)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_whose_join_would_have_too_many_threads_are_refused(D):
+    """256 threads to 8 rows (head dim 128): 2^27 - 7 rows would be 2^32."""
+    lib = _lib.load()
+    fn = lib.hlm_attn_cached_fwd_workspace_bytes
+    some = P(0x1000)
+    for rows, ok in (((1 << 27) - 8, True), ((1 << 27) - 7, False), ((1 << 27) - 1, False)):
+        n = fn(1, rows, 1, 1, D, 64, some, 0, None, 5000, 64)
+        assert n % (rows * (D + 2) * 4) == 0 and n > 0 if ok else n == -2
+    assert b"too many query rows" in lib.hlm_attn_last_error()
