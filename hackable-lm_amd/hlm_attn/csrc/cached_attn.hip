@@ -852,7 +852,7 @@ hipError_t launch(const CachedAttnArgs& p, hipStream_t stream) {
 //    workgroup: the larger tile costs less a row, the smaller spreads better.
 //  * Partial sums cost 3.0 for the second kernel (the prefix's are joined with
 //    the own ones in any case) and are written and read at 4.5 TB/s.
-// `others` workgroups run beside these.
+// `others` workgroups run beside these; `most` is the largest variant.
 struct Split {
   int variant, tiles, splits;
   double us;
@@ -861,10 +861,10 @@ struct Split {
 constexpr double kJoinUs = 3.0;
 
 template <int D>
-Split choose(int64_t rows, int64_t units, int64_t blocks, int64_t all_rows, bool joined, int64_t others) {
+Split choose(int64_t rows, int64_t units, int64_t blocks, int64_t all_rows, bool joined, int64_t others, int most = 2) {
   Split best{0, 1, 1, 1e300};
   const double row_us = (D + 2) * 8 / 4.5e6;
-  for (int v = rows <= 16 ? 0 : 1; v <= (rows <= 16 ? 0 : rows <= 64 ? 1 : 2); ++v) {
+  for (int v = rows <= 16 ? 0 : 1; v <= (rows <= 16 ? 0 : rows <= 64 ? 1 : most); ++v) {
     const int64_t tiles = (rows + tile_rows(v) - 1) / tile_rows(v), items = units * tiles;
     for (int n : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
       if (n > blocks && n > 1) break;
@@ -900,7 +900,11 @@ int64_t plan_cached_attn(CachedAttnArgs& p, int64_t keys) {
   p.prefix_tiles = p.prefix_splits = 0;
   if (p.P > 0) {
     const int64_t seen = std::min<int64_t>(p.P, p.window);  // own tokens stand behind the prefix
-    Split pre = choose<D>(rows * p.B, p.Hkv, (seen + 63) / 64 + 1, all, true, units * own.tiles * own.splits);
+    // Beside own tiles of 16 rows the model has the prefix's 128-row ones ahead in one
+    // shape of 2500, where they are not: 6 x 12 tokens over 11351, 16 heads of 64,
+    // 26.4 us with them and 26.5 with 64 rows; 23 tokens over 24516, 32 heads of 128 in
+    // 8 groups, 51.6 and 47.0; 202 x 2 over 476 in one group, 32.3 and 27.9.
+    Split pre = choose<D>(rows * p.B, p.Hkv, (seen + 63) / 64 + 1, all, true, units * own.tiles * own.splits, own.variant == 0 ? 1 : 2);
     // one kernel for both: 128-row tiles of a sequence's rows need them of the prefix's
     if (pre.variant < own.variant) pre.variant = own.variant, pre.tiles = (int)((rows * p.B + 127) / 128);
     // Or each sequence's rows over both: the prefix is read once per sequence, mostly
@@ -940,7 +944,6 @@ hipError_t launch_cached_attn(const CachedAttnArgs& p, hipStream_t stream) {
     case 4 * 2 - 1: return launch<D, 2, -1>(p, stream);
     case 4 * 0 + 0: return launch<D, 0, 0>(p, stream);
     case 4 * 0 + 1: return launch<D, 0, 1>(p, stream);
-    case 4 * 0 + 2: return launch<D, 0, 2>(p, stream);
     case 4 * 1 + 1: return launch<D, 1, 1>(p, stream);
     case 4 * 1 + 2: return launch<D, 1, 2>(p, stream);
     case 4 * 2 + 2: return launch<D, 2, 2>(p, stream);
