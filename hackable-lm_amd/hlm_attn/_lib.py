@@ -46,6 +46,7 @@ _SPAN = [_P, _I, _P]  # starts (or null), start, counts (or null)
 SIGNATURES["hlm_attn_cache_write"] = (_I, [_P, _P, _S, _S, _P, _P, _P, _P, _I, *_SPAN, _I, _I, _I, _I, _P])
 SIGNATURES["hlm_attn_cache_read"] = (_I, [_P, _P, _P, _P, _I, _P, _P, *_SPAN, _I, _I, _I, _I, _P])
 SIGNATURES["hlm_attn_cached_fwd_workspace_bytes"] = (_I64, [_I] * 6 + _SPAN + [_I, _I])
+SIGNATURES["hlm_attn_cached_fwd_plan"] = (_I, [_I] * 6 + _SPAN + [_I, _I, ctypes.POINTER(ctypes.c_int32)])
 SIGNATURES["hlm_attn_cached_fwd"] = (
     _I, [_P, _S, _P, _P, _P, _P, _P, _I, *_SPAN, _P, _P, _P, _P, _I, _I, *[_I] * 6, _F, _P, _I64, _P])
 SIGNATURES["hlm_residual_rms_norm_fwd"] = (_I, [_P, _P, _P, _P, _I64, _I, _F, _P])

@@ -743,6 +743,18 @@ int64_t hlm_attn_cached_fwd_workspace_bytes(int B, int T, int H, int Hkv, int D,
   return floats * 4;
 }
 
+int hlm_attn_cached_fwd_plan(int B, int T, int H, int Hkv, int D, int slots, const int32_t* starts, int start,
+                             const int32_t* counts, int prefix_length, int window, int32_t* plan) {
+  g_last_error[0] = '\0';
+  if (plan == nullptr) return fail(HLM_ATTN_EINVAL, "plan is a null pointer");
+  hlm::CachedAttnArgs a{};
+  int64_t floats = 0;
+  if (const int rc = plan_cached(a, floats, B, T, H, Hkv, D, slots, starts, start, counts, prefix_length, window)) return rc;
+  const int32_t p[6] = {a.variant, a.own_tiles, a.own_splits, a.prefix_variant, a.prefix_tiles, a.prefix_splits};
+  std::copy(p, p + 6, plan);
+  return HLM_ATTN_OK;
+}
+
 int hlm_attn_cached_fwd(const void* q, const int64_t* q_strides, void* o, const void* cache_k, const void* cache_v,
                         const float* k_scale, const float* v_scale, int slots, const int32_t* starts, int start,
                         const int32_t* counts, const void* prefix_k, const void* prefix_v, const float* prefix_k_scale,

@@ -372,6 +372,14 @@ int hlm_attn_cached_fwd(const void* q, const int64_t* q_strides, void* o, const 
  * of starts and counts only whether they are null; touches no device. */
 int64_t hlm_attn_cached_fwd_workspace_bytes(int B, int T, int H, int Hkv, int D, int slots, const int32_t* starts, int start,
                                             const int32_t* counts, int prefix_length, int window);
+/* How that call would share out its work: plan[0 .. 5] = the kernel of the own
+ * keys (0: tiles of 16 query rows whose waves share the keys; 1, 2: 64 and 128
+ * rows, which the waves share), its tiles per sequence and kv head, its splits
+ * of their keys; the prefix's kernel (-1: no prefix; -2: the sequences' tiles
+ * take the prefix's keys with their own, in one pass), tiles per kv head, and
+ * splits.  All zeros for empty calls.  Touches no device. */
+int hlm_attn_cached_fwd_plan(int B, int T, int H, int Hkv, int D, int slots, const int32_t* starts, int start,
+                             const int32_t* counts, int prefix_length, int window, int32_t* plan);
 
 /* Message describing the last failed call on this thread ("" if none). */
 const char* hlm_attn_last_error(void);

@@ -675,3 +675,84 @@ def test_attention_over_vmap_is_that_of_its_parts():
             assert torch.equal(a, hlm_attn.cached_attention_hip(b.cuda(), cache, 100))
         with pytest.raises(RuntimeError, match="[Bb]atching rule"):
             torch.func.vmap(lambda x: (hlm_attn.kv_cache_write_hip(cache, x, x, 0), x)[1])(_rand(g, 3, 2, 1, 2, 64).cuda())
+
+
+# --- each kernel of the plan ------------------------------------------------------------------
+
+
+def plan_of(B, T, H, Hkv, D, slots, prefix, window):
+    """The plan's kernels, with places on the device: of the own keys and of the prefix (see hlm_attn_cached_fwd_plan)."""
+    import ctypes
+
+    from hlm_attn import _lib
+
+    plan = (ctypes.c_int32 * 6)()
+    assert _lib.load().hlm_attn_cached_fwd_plan(B, T, H, Hkv, D, slots, ctypes.c_void_p(16), 0, None, prefix, window or 0, plan) == 0
+    return plan[0], plan[3]
+
+
+def check_rows(out, q, k, v, starts, counts, rows, window=None, prefix=None, scale=None):
+    """check_attention of the rows (sequence, token) alone, each as a sequence of one token."""
+    out = out.cpu()
+    for b, t in rows:
+        check_attention(out[b : b + 1, t : t + 1], q[b : b + 1, t : t + 1], *([x[b : b + 1] for x in pair] for pair in (k, v)),
+                        [starts[b] + t], [int(t < counts[b])], window, scale, prefix)
+
+
+KERNELS = [
+    # own kernel, prefix's (-1: no prefix; -2: the prefix's keys with the own ones), B, T, H, Hkv, D, capacity, window, P
+    (0, 0, 1, 1, 3, 1, 64, 128, None, 852),
+    (0, 0, 2, 1, 3, 1, 64, 960, 964, 55),
+    (0, 0, 1, 1, 4, 1, 64, 64, None, 4650),
+    (0, 0, 4, 1, 3, 1, 128, 64, None, 451),
+    (0, 0, 2, 1, 3, 1, 128, 512, 460, 39),
+    (0, 1, 66, 1, 4, 4, 64, 64, None, 424),
+    (0, 1, 55, 1, 3, 1, 64, 128, 933, 1127),
+    (0, 1, 64, 1, 12, 4, 64, 512, None, 8000),
+    (0, 1, 8, 4, 3, 1, 128, 128, None, 393),
+    (0, 1, 5, 4, 3, 1, 128, 256, 489, 265),
+    (1, 1, 2, 28, 3, 1, 64, 128, None, 194),
+    (1, 1, 6, 12, 3, 1, 64, 128, 271, 194),
+    (1, 1, 5, 73, 3, 1, 128, 192, None, 72),
+    (1, 1, 7, 6, 3, 1, 128, 64, 330, 267),
+    (1, 2, 35, 36, 4, 4, 64, 64, None, 5344),
+    (1, 2, 93, 9, 6, 2, 64, 64, None, 7000),
+    (1, 2, 108, 23, 3, 1, 128, 256, None, 2314),
+    (1, 2, 53, 14, 4, 2, 128, 640, 6606, 10190),
+    (2, 2, 29, 185, 3, 1, 64, 1216, None, 845),
+    (2, 2, 36, 98, 4, 4, 64, 768, 884, 269),
+    (2, 2, 34, 159, 3, 1, 128, 1216, None, 426),
+    (2, 2, 10, 209, 8, 1, 128, 960, 1160, 311),
+    (2, -1, 109, 37, 8, 4, 64, 64, None, 0),
+    (2, -1, 1, 5000, 12, 4, 64, 5056, None, 0),
+    (2, -1, 101, 43, 8, 4, 64, 64, 20, 0),
+    (2, -1, 101, 23, 12, 4, 128, 64, None, 0),
+    (2, -1, 102, 25, 12, 4, 128, 64, 9, 0),
+    (2, -1, 1, 5000, 12, 4, 128, 5056, 1000, 0),
+    (2, -2, 32, 65, 16, 16, 64, 192, 80, 70),
+    (2, -2, 32, 65, 16, 16, 128, 192, None, 70),
+]
+
+
+@pytest.mark.parametrize("own,shared,B,T,H,Hkv,D,capacity,window,P", KERNELS)
+def test_each_kernel_of_the_plan(own, shared, B, T, H, Hkv, D, capacity, window, P):
+    """A ragged batch at places of its own, the slots behind the prefix holding anything: forty rows of it."""
+    assert plan_of(B, T, H, Hkv, D, capacity, P, window) == (own, shared)
+    g = torch.Generator().manual_seed(B * T + P)
+    cache, (k, v) = filled(g, B, capacity, Hkv, D)
+    prefix = pre = None
+    if P:
+        pre, whole = filled(g, 1, P, Hkv, D)
+        for scale, fill in ((pre.k_scale, float("nan")), (pre.v_scale, float("inf"))):
+            scale[:, :, P:] = fill
+        prefix = [(c[:, :, :P], s[:, :, :P]) for c, s in whole]
+    q = _rand(g, B, T, H, D, scale=1.5)
+    starts = [b * 37 % (capacity - T + 1) for b in range(B)]
+    starts[-1] = capacity - T
+    counts = [T - b * 5 % (T + 1) for b in range(B)]
+    out = hlm_attn.cached_attention_hip(q.cuda(), cache, int32(starts), int32(counts), window, prefix=pre, prefix_length=P)
+    ends = [(b, t) for b in (0, 1 % B, B - 1) for t in {0, counts[b] - 1, min(T - 1, counts[b]), T // 2, T - 1} if t >= 0]
+    some = [(int(b), int(t)) for b, t in zip(torch.randint(B, (25,), generator=g), torch.randint(T, (25,), generator=g))]
+    check_rows(out, q, k, v, starts, counts, ends + some, window, prefix)
+    dead = torch.arange(T)[None] >= torch.tensor(counts)[:, None]
+    assert not out.cpu()[dead].any() and torch.isfinite(out).all()

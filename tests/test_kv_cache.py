@@ -444,3 +444,63 @@ def test_rows_whose_join_would_have_too_many_threads_are_refused(D):
         n = fn(1, rows, 1, 1, D, 64, some, 0, None, 5000, 64)
         assert n % (rows * (D + 2) * 4) == 0 and n > 0 if ok else n == -2
     assert b"too many query rows" in lib.hlm_attn_last_error()
+
+
+# --- the plan -----------------------------------------------------------------------------
+
+
+def plan_of(B, T, H, Hkv, D, slots, prefix, window, starts=P(0x1000), start=0):
+    """(own kernel, tiles, splits, prefix kernel, tiles, splits) of hlm_attn_cached_fwd."""
+    lib = _lib.load()
+    plan = (ctypes.c_int32 * 6)()
+    assert lib.hlm_attn_cached_fwd_plan(B, T, H, Hkv, D, slots, starts, start, None, prefix, window, plan) == 0
+    return tuple(plan)
+
+
+def test_plan_of_long_and_short_prefixes():
+    """64 samples: a prefix of 60 goes with the own keys, without a join; a long one is read once for all of them."""
+    fn = _lib.load().hlm_attn_cached_fwd_workspace_bytes
+    some = P(0x1000)
+    assert fn(64, 1, 12, 12, 64, 64, some, 0, None, 60, 0) == 0
+    assert plan_of(64, 1, 12, 12, 64, 64, 60, 0) == (0, 1, 1, -2, 0, 0)
+    assert plan_of(64, 1, 12, 12, 64, 64, 8000, 0)[3] == 1
+    assert fn(64, 1, 12, 12, 64, 64, some, 0, None, 8000, 0) >= 2 * 64 * 12 * (64 + 2) * 4
+    assert plan_of(1, 1, 4, 4, 64, 64, 0, 0) == (0, 1, 1, -1, 0, 0)
+    assert plan_of(0, 1, 4, 4, 64, 64, 0, 0) == (0,) * 6
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_plan_names_a_kernel_that_exists_and_agrees_with_the_workspace(D):
+    """The own keys' kernel alone, with the prefix in one pass, or beside the prefix's: (0, 0), (0, 1), (1, 1), (1, 2), (2, 2)."""
+    import random
+
+    fn = _lib.load().hlm_attn_cached_fwd_workspace_bytes
+    rng = random.Random(D)
+    seen = set()
+    for _ in range(4000):
+        H = rng.choice((1, 3, 4, 12, 16))
+        Hkv = rng.choice([g for g in (1, 2, 3, 4, 16) if H % g == 0])
+        B, T = int(2 ** rng.uniform(0, 8)), int(2 ** rng.choice((0, rng.uniform(0, 11))))
+        slots, prefix, window = 64 * int(2 ** rng.uniform(0, 10)), rng.choice((0, int(2 ** rng.uniform(0, 14)))), rng.choice((0, 1, 700))
+        v, tiles, splits, vp, ptiles, psplits = plan_of(B, T, H, Hkv, D, slots, prefix, window)
+        seen.add((v, vp))
+        rows = T * (H // Hkv)
+        assert tiles == -(-rows // (16, 64, 128)[v]) and 1 <= splits <= 64
+        if vp >= 0:
+            assert prefix and ptiles == -(-rows * B // (16, 64, 128)[vp]) and 1 <= psplits <= 64
+        else:
+            assert vp == (-2 if prefix else -1) and ptiles == psplits == 0
+        n = splits + psplits
+        assert fn(B, T, H, Hkv, D, slots, P(0x1000), 0, None, prefix, window) == (0 if n == 1 else n * B * T * H * (D + 2) * 4)
+    assert seen <= {(v, vp) for v in (0, 1, 2) for vp in (-1, -2)} | {(0, 0), (0, 1), (1, 1), (1, 2), (2, 2)}
+    assert len(seen) >= 8
+
+
+def test_plan_refuses_what_the_call_refuses():
+    lib = _lib.load()
+    plan = (ctypes.c_int32 * 6)()
+    args = lambda **kw: [{**dict(B=1, T=1, H=2, Hkv=2, D=64, slots=64, starts=None, start=0, counts=None, prefix=0, window=0), **kw}[n]
+                         for n in ("B", "T", "H", "Hkv", "D", "slots", "starts", "start", "counts", "prefix", "window")]
+    assert lib.hlm_attn_cached_fwd_plan(*args(), None) == -1 and b"plan" in lib.hlm_attn_last_error()
+    for kw, code in ((dict(D=96), -2), (dict(H=3), -1), (dict(slots=65), -1), (dict(start=64), -1), (dict(prefix=-1), -1)):
+        assert lib.hlm_attn_cached_fwd_plan(*args(**kw), plan) == code
