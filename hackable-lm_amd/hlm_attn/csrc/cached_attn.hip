@@ -42,8 +42,10 @@
 // Numerics.  q is scaled by a power of two to at most 2 per row and then held
 // in fp16 (exact but for values 2^-14 of the row's largest and below, whose
 // error is 2^-25 of it); whole numbers are exact; products and sums are fp32.
-// p_j vs_j is rounded to fp16 relative to the largest vs that the row has seen
-// so far, 2^11 at p = 1: 11 bits for weights above 2^-25, and none above 2^-36 is lost.
+// p_j vs_j is rounded to fp16 relative to the largest vs that the row has seen so
+// far, 2^11 at p = 1, or to 2^8 times the largest p_j vs_j if that is less (a key
+// of little weight may have a value far above the others): 11 bits for weights
+// above 2^-25 of it, and none above 2^-36 is lost.
 // Neither sum can pass fp32 while keys are below 2^119 (q.k_j with q at 2, D = 128)
 // and values below 2^100 (2^24 keys at up to 2^3).
 #include <cmath>
@@ -58,10 +60,15 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 constexpr float kWeightTop = 2048.f;  // a probability of 1 as fp16
-// The running maximum is moved only when a score passes it by 2^3, the value
-// scales that weights are relative to only when one passes the smallest by 2:
-// weights reach 2^15, within fp16, and the sums stay where they are meanwhile.
+// The running maximum is moved only when a score passes it by 2^3, and what weights
+// are relative to then or when a value scale passes the smallest by 2: weights
+// reach 2^15, within fp16, and the sums stay where they are meanwhile.
 constexpr float kSlack = 3.f;
+// What weights are relative to stays within this of the row's largest weight:
+// keys that get 2^-8 of the row's attention, beside one that takes it all with a
+// value as much smaller, still leave it where it is for all rows of a wave.
+constexpr float kWeightRoom = 256.f;
+constexpr float kSmallest = 1.17549435e-38f;  // 2^-126
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -203,10 +210,11 @@ struct Rows {
   f16x8 q[NT][C][2];
   float rs[NT];             // scale log2(e) and q's power of two
   float mt[NT], l[NT];      // running maximum of (q.kc) ks, sum
-  // The value scale that each row's weights are relative to: the largest that the
-  // row has seen (0: none yet), and its inverse.  The rows' smallest and largest,
-  // for the wave, and the largest's inverse: mostly they are the same.
-  float vtop[NT], per[NT], vlow, vhigh, per_vhigh;
+  // The value scale that each row's weights are relative to (0: none yet), and a
+  // weight p vs that the row has seen, its largest when they were last looked at.
+  // The scales' smallest and largest, for the wave, and the largest's inverse:
+  // mostly they are the same.
+  float ref[NT], heavy[NT], vlow, vhigh, per_vhigh;
   f32x4 o[NT][DT];          // o^T: dims 16 d + 4 g + i of row n
 
   // The rows r0 .. of a unit.  Queries are loaded before the places are known
@@ -272,7 +280,7 @@ struct Rows {
 #pragma unroll
           for (int e = 0; e < 8; ++e) q[nt][c][h][e] = (_Float16)((float)x[nt][c][h][e] * down);
       mt[nt] = -__builtin_inff();
-      l[nt] = vtop[nt] = per[nt] = 0.f;
+      l[nt] = ref[nt] = heavy[nt] = 0.f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -300,7 +308,7 @@ struct Rows {
       }
       if (k0 + lane_key(lane) < first || k0 + lane_key(lane) > min(last, end)) vs = 0.f;
     }
-    if (__any(vs > 2.f * vlow)) raise_vtop(sc, vs);
+    bool light = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = sc[nt][0][0];
@@ -311,6 +319,8 @@ struct Rows {
         const float alpha = m > mt[nt] ? __builtin_amdgcn_exp2f((mt[nt] - m) * rs[nt]) : 1.f;
         mt[nt] = m;
         l[nt] *= alpha;
+        heavy[nt] *= alpha;
+        light |= ref[nt] > kWeightRoom * heavy[nt];
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[nt][d] *= alpha;
       }
@@ -324,6 +334,7 @@ struct Rows {
       }
       l[nt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
+    if (__any(light || vs > 2.f * vlow)) settle(sc, vs, whole);
     if (whole && vlow == vhigh) {
       const float rel = vs * per_vhigh * kWeightTop;  // 1 / vhigh <= 2^126: kWeightTop times it may be beyond fp32
       each<16>([&](auto e) {
@@ -332,6 +343,9 @@ struct Rows {
         for (int nt = 0; nt < NT; ++nt) w[nt][e / 8][e % 8] = (_Float16)(sc[nt][e / 4][e % 4] * f);
       });
     } else {  // a masked key's scale may be anything
+      float per[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) per[nt] = __builtin_amdgcn_rcpf(fmaxf(ref[nt], kSmallest));  // 0 while all scales were
       each<16>([&](auto e) {
         const float f = row_lane<e>(vs);
 #pragma unroll
@@ -343,28 +357,37 @@ struct Rows {
     }
   }
 
-  // Raises the rows' value scales to those that they see in this block (rows that
-  // do not see a key, whose score is -infinity then, keep clear of its scale).
-  __device__ __forceinline__ void raise_vtop(const f32x4 sc[NT][4], float vs) {
+  // Sets what the rows' weights are relative to, by the block's probabilities p and
+  // value scales: the largest scale with a weight, or kWeightRoom times the row's
+  // largest weight if that is less (keys that a row does not see have p = 0, and it
+  // keeps clear of their scales).  A weight is then at most 2^3 kWeightTop, in later
+  // blocks 2^4, since they come here if a scale passes 2 ref; and o, in its old
+  // units at most as large as in the new ones, cannot pass fp32.
+  __device__ __forceinline__ void settle(const f32x4 p[NT][4], float vs, bool whole) {
     float low = __builtin_inff(), high = 0.f;
+    const float highest = whole ? over_groups(over_lanes(vs, Max()), Max()) : 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float top = 0.f;
-      each<16>([&](auto e) {
-        const float f = row_lane<e>(vs);
-        top = fmaxf(top, sc[nt][e / 4][e % 4] > -__builtin_inff() ? f : 0.f);
-      });
-      top = over_groups(top, Max());
-      if (top > vtop[nt]) {
-        const float f = vtop[nt] / top;
-        vtop[nt] = top;
-        per[nt] = 1.f / top;
+      float scale = highest, weight = 0.f;
+      each<16>([&](auto e) { weight = fmaxf(weight, p[nt][e / 4][e % 4] * row_lane<e>(vs)); });  // a NaN is passed over
+      if (!whole) {
+        each<16>([&](auto e) {
+          const float f = row_lane<e>(vs);
+          scale = fmaxf(scale, p[nt][e / 4][e % 4] > 0.f ? f : 0.f);
+        });
+        scale = over_groups(scale, Max());
+      }
+      heavy[nt] = fmaxf(heavy[nt], over_groups(weight, Max()));
+      const float to = fmaxf(kSmallest, fminf(fmaxf(ref[nt], scale), kWeightRoom * heavy[nt]));
+      if (ref[nt] > 0.f && to != ref[nt]) {  // before the first weight o is zero
+        const float f = fminf(3e38f, ref[nt] / to);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[nt][d] *= f;
       }
+      ref[nt] = to;
       if (hi[nt] >= lo[nt]) {
-        low = fminf(low, vtop[nt]);
-        high = fmaxf(high, vtop[nt]);
+        low = fminf(low, ref[nt]);
+        high = fmaxf(high, ref[nt]);
       }
     }
     vlow = uniform(over_lanes(low, Min()));
@@ -515,7 +538,7 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
     const float f = mine == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mine - m) / kWeightTop;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = rows.o[nt][d] * f * rows.vtop[nt];
+      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = rows.o[nt][d] * f * rows.ref[nt];
   }
   __syncthreads();
   constexpr int U = D / 4;
@@ -686,7 +709,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
         bf16x4 y = {};
         if (real)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = (bf16)(rows.o[nt][d][i] * f * rows.vtop[nt]);
+          for (int i = 0; i < 4; ++i) y[i] = (bf16)(rows.o[nt][d][i] * f * rows.ref[nt]);
         *reinterpret_cast<bf16x4*>(p.o + out * D + 16 * d + 4 * g) = y;
       }
     } else {
@@ -701,7 +724,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
       if (has)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          __builtin_nontemporal_store(rows.o[nt][d] / kWeightTop * rows.vtop[nt],
+          __builtin_nontemporal_store(rows.o[nt][d] / kWeightTop * rows.ref[nt],
                                       reinterpret_cast<f32x4*>(p.part_o + at * D + 16 * d + 4 * g));
     }
   }

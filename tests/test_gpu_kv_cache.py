@@ -756,3 +756,87 @@ def test_each_kernel_of_the_plan(own, shared, B, T, H, Hkv, D, capacity, window,
     check_rows(out, q, k, v, starts, counts, ends + some, window, prefix)
     dead = torch.arange(T)[None] >= torch.tensor(counts)[:, None]
     assert not out.cpu()[dead].any() and torch.isfinite(out).all()
+
+
+# --- values far above others, with little weight ----------------------------------------------
+
+
+def check_by_weight(out, q, k, v, starts, counts, window=None, scale=None, prefix=None):
+    """check_attention with the fp16 weights' absolute error relative to the row's largest weight p vs instead of its largest
+    value scale: what weights are relative to is at most 2^8 of the former, so one is off by at most 2^-36 2^8 of it, times a
+    whole number of at most 127."""
+    o, a, reach, _ = oracle.attention(q, k, v, starts, counts, window, scale, prefix)
+    B, T, H, D = q.shape
+    scale = D**-0.5 if scale is None else scale
+    P = prefix[0][0].shape[2] if prefix else 0
+    n = k[0].shape[2] + P
+    heavy = torch.zeros(B, T, H, dtype=torch.float64)
+    for b in range(B):
+        for h in range(H):
+            g = h // (H // k[0].shape[1])
+            kr, ks, vs = (torch.cat([x[i][0, g] for x in (prefix[j],)] + [own[i][b, g]]) if P else own[i][b, g]
+                          for own, i, j in ((k, 0, 0), (k, 1, 0), (v, 1, 1)))
+            s = (q[b, :, h].double() @ kr.double().T) * ks * scale
+            lag = (torch.arange(T) + starts[b] + P)[:, None] - torch.arange(n)
+            s = s.masked_fill((lag < 0) | (lag >= (window or n + 1)), -float("inf"))
+            heavy[b, :, h] = (torch.softmax(s, -1) * vs).amax(-1)
+    kmax = max((c[0].abs().sum(-1) * c[1]).max().item() for c in ([k] + ([prefix[0]] if prefix else [])))
+    e_s = (D + 4) * 2.0**-24 * reach + 2.0**-23 * q.double().abs().amax(-1) * kmax * scale
+    rel = 4 * e_s + 2.0**-20 + 2.0**-11 + n * 2.0**-23
+    tol = 2.0**-8 * o.abs() + (a * rel[..., None] + (n * 127 * 2.0**-28 * heavy)[..., None]) * (1 + 2.0**-8)
+    err = (out.double().cpu() - o).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"error {(err / tol).max().item():.3f} of its bound"
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,window", [(1, None), (5, None), (5, 100), (60, None), (60, 70), (130, 90)])
+def test_a_visible_value_far_above_the_others_with_little_weight(D, T, window):
+    """Values near 1, and single ones of 2^40 whose keys' logits are 40 and 100 below: the others keep their bits, wherever
+    the large ones stand, in the cache and in a prefix."""
+    g = torch.Generator().manual_seed(T)
+    S, start, H, P = 320, 150, 4, 100
+    for below in (40.0, 100.0):
+        for spots in ((start,), (0, 70), (start - 3, start - 60, 5)):
+            q = _rand(g, 1, T, H, D)
+            q[..., 0] = 8.0
+            k, v = _rand(g, 1, S, 2, D), _rand(g, 1, S, 2, D)
+            k[..., 0] = 0.0
+            for at in spots:
+                k[0, at, :, 0] = -below * D**0.5 / 8
+                v[0, at] = (v[0, at].float() * 2.0**40).bfloat16()
+            cache, (kp, vp) = filled(g, 1, S, 2, D, k, v)
+            out = hlm_attn.cached_attention_hip(q.cuda(), cache, start, None, window)
+            check_by_weight(out, q, kp, vp, [start], [T], window)
+            pre, whole = filled(g, 1, P, 2, D, *(torch.nn.functional.pad(x[:, :P], (0, 0, 0, 0, 0, 128 - P)) for x in (k, v)))
+            prefix = [(c[:, :, :P], s[:, :, :P]) for c, s in whole]
+            out = hlm_attn.cached_attention_hip(q.cuda(), cache, start, None, window, prefix=pre, prefix_length=P)
+            check_by_weight(out, q, kp, vp, [start], [T], window, prefix=prefix)
+
+
+@pytest.mark.parametrize("T,H", [(1, 2), (40, 2), (300, 12)])
+def test_weights_and_values_over_many_powers_of_two(T, H):
+    """Logits that rise and fall by tens along the keys, values of 10^-6 to 10^6: each row to its own weights."""
+    g = torch.Generator().manual_seed(T)
+    S, D = 1024, 64
+    q = _rand(g, 1, T, H, D)
+    q[..., 0] = 8.0
+    k = _rand(g, 1, S, 2, D)
+    k[0, :, :, 0] = (torch.randn(S, 2, generator=g).cumsum(0) * 3).bfloat16()
+    v = (torch.randn(1, S, 2, D, generator=g) * 10.0 ** torch.randint(-6, 7, (1, S, 2, 1), generator=g)).bfloat16()
+    cache, (kp, vp) = filled(g, 1, S, 2, D, k, v)
+    out = hlm_attn.cached_attention_hip(q.cuda(), cache, S - T)
+    check_by_weight(out, q, kp, vp, [S - T], [T])
+
+
+def test_one_key_that_takes_it_all_with_a_small_value():
+    """A first key with nearly all the weight and a value of 2^-20, as models learn: the others' share is kept."""
+    g = torch.Generator().manual_seed(23)
+    for T in (1, 20, 100):
+        q, k, v = _rand(g, 1, T, 4, 64), _rand(g, 1, 512, 2, 64), _rand(g, 1, 512, 2, 64)
+        q[..., 0], k[..., 0] = 8.0, 0.0
+        k[0, 0, :, 0] = 9.0
+        v[0, 0] = (v[0, 0].float() * 2.0**-20).bfloat16()
+        cache, (kp, vp) = filled(g, 1, 512, 2, 64, k, v)
+        out = hlm_attn.cached_attention_hip(q.cuda(), cache, 512 - T)
+        check_by_weight(out, q, kp, vp, [512 - T], [T])
