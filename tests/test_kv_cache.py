@@ -504,3 +504,55 @@ def test_plan_refuses_what_the_call_refuses():
     assert lib.hlm_attn_cached_fwd_plan(*args(), None) == -1 and b"plan" in lib.hlm_attn_last_error()
     for kw, code in ((dict(D=96), -2), (dict(H=3), -1), (dict(slots=65), -1), (dict(start=64), -1), (dict(prefix=-1), -1)):
         assert lib.hlm_attn_cached_fwd_plan(*args(**kw), plan) == code
+
+
+# --- the library's kernels --------------------------------------------------------------------
+
+
+def _kernels_of_library():
+    """The metadata of each kernel in the built library, by name: the notes of the code objects in its offload bundles."""
+    import struct
+
+    msgpack = pytest.importorskip("msgpack")
+    data = _lib.LIB_PATH.read_bytes()
+    found, magic = {}, b"__CLANG_OFFLOAD_BUNDLE__"
+    at = data.find(magic)
+    while at >= 0:
+        (n,) = struct.unpack_from("<Q", data, at + 24)
+        p = at + 32
+        for _ in range(n):
+            offset, size, length = struct.unpack_from("<QQQ", data, p)
+            target = data[p + 24 : p + 24 + length]
+            p += 24 + length
+            if b"gfx950" not in target:
+                continue
+            elf = data[at + offset : at + offset + size]
+            (sections,) = struct.unpack_from("<Q", elf, 0x28)
+            entry, count = struct.unpack_from("<HH", elf, 0x3A)
+            for i in range(count):
+                kind, _, _, start, length_ = struct.unpack_from("<IQQQQ", elf, sections + i * entry + 4)
+                if kind != 7:  # a note
+                    continue
+                name, desc, _ = struct.unpack_from("<III", elf, start)
+                text = start + 12 + (name + 3) // 4 * 4
+                for k in msgpack.unpackb(elf[text : text + desc], strict_map_key=False)["amdhsa.kernels"]:
+                    found[k[".name"]] = k
+        at = data.find(magic, at + 1)
+    return found
+
+
+def test_the_attention_kernels_fit_their_registers():
+    """No scratch memory anywhere, four waves a SIMD (128 registers) for the 16- and 64-row kernels at head dim 64, and no
+    kernel that no plan names."""
+    import re
+
+    seen = set()
+    for name, k in _kernels_of_library().items():
+        if "cached_attn_kernel" not in name:
+            continue
+        D, v, vp = (int(x.replace("n", "-")) for x in re.search(r"cached_attn_kernelILi(\d+)ELi(\d+)ELi(n?\d+)EE", name).groups())
+        seen.add((D, v, vp))
+        assert k[".private_segment_fixed_size"] == 0 and k[".vgpr_spill_count"] == 0, name
+        assert k[".vgpr_count"] + k.get(".agpr_count", 0) <= (128 if D == 64 and v < 2 and vp < 2 else 256), name
+    assert seen == {(D, v, vp) for D in (64, 128) for v, vp in
+                    [(v, vp) for v in (0, 1, 2) for vp in (-1, -2)] + [(0, 0), (0, 1), (1, 1), (1, 2), (2, 2)]}
