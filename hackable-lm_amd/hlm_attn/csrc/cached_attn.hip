@@ -42,10 +42,10 @@
 // Numerics.  q is scaled by a power of two to at most 2 per row and then held
 // in fp16 (exact but for values 2^-14 of the row's largest and below, whose
 // error is 2^-25 of it); whole numbers are exact; products and sums are fp32.
-// p_j vs_j is rounded to fp16 relative to the largest vs that the row has seen so
-// far, 2^11 at p = 1, or to 2^8 times the largest p_j vs_j if that is less (a key
-// of little weight may have a value far above the others): 11 bits for weights
-// above 2^-25 of it, and none above 2^-36 is lost.
+// p_j vs_j is rounded to fp16 relative to the largest vs that the wave's rows have
+// seen so far, 2^11 at p = 1, or to 2^8 times the row's own largest p_j vs_j if that
+// is less (a key of little weight may have a value far above the others): 11 bits
+// for weights above 2^-25 of it, and none above 2^-36 is lost.
 // Neither sum can pass fp32 while keys are below 2^119 (q.k_j with q at 2, D = 128)
 // and values below 2^100 (2^24 keys at up to 2^3).
 #include <cmath>
@@ -334,7 +334,7 @@ struct Rows {
       }
       l[nt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    if (__any(light || vs > 2.f * vlow)) settle(sc, vs, whole);
+    if (__any(light || vs > 2.f * vlow)) settle(sc, vs);
     if (whole && vlow == vhigh) {
       const float rel = vs * per_vhigh * kWeightTop;  // 1 / vhigh <= 2^126: kWeightTop times it may be beyond fp32
       each<16>([&](auto e) {
@@ -358,25 +358,18 @@ struct Rows {
   }
 
   // Sets what the rows' weights are relative to, by the block's probabilities p and
-  // value scales: the largest scale with a weight, or kWeightRoom times the row's
-  // largest weight if that is less (keys that a row does not see have p = 0, and it
-  // keeps clear of their scales).  A weight is then at most 2^3 kWeightTop, in later
-  // blocks 2^4, since they come here if a scale passes 2 ref; and o, in its old
-  // units at most as large as in the new ones, cannot pass fp32.
-  __device__ __forceinline__ void settle(const f32x4 p[NT][4], float vs, bool whole) {
+  // value scales vs (0 for keys that no row sees): the largest scale, or kWeightRoom
+  // times the row's largest weight if that is less (so a row keeps clear of scales
+  // that only others see; its own p is 0 there).  A weight is then at most 2^3
+  // kWeightTop, in later blocks 2^4, since they come here if a scale passes 2 ref;
+  // and o, in its old units at most as large as in the new ones, cannot pass fp32.
+  __device__ __forceinline__ void settle(const f32x4 p[NT][4], float vs) {
     float low = __builtin_inff(), high = 0.f;
-    const float highest = whole ? over_groups(over_lanes(vs, Max()), Max()) : 0.f;
+    const float scale = over_groups(over_lanes(vs, Max()), Max());
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float scale = highest, weight = 0.f;
+      float weight = 0.f;
       each<16>([&](auto e) { weight = fmaxf(weight, p[nt][e / 4][e % 4] * row_lane<e>(vs)); });  // a NaN is passed over
-      if (!whole) {
-        each<16>([&](auto e) {
-          const float f = row_lane<e>(vs);
-          scale = fmaxf(scale, p[nt][e / 4][e % 4] > 0.f ? f : 0.f);
-        });
-        scale = over_groups(scale, Max());
-      }
       heavy[nt] = fmaxf(heavy[nt], over_groups(weight, Max()));
       const float to = fmaxf(kSmallest, fminf(fmaxf(ref[nt], scale), kWeightRoom * heavy[nt]));
       if (ref[nt] > 0.f && to != ref[nt]) {  // before the first weight o is zero
@@ -751,9 +744,9 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int ti
 // V, VP: variants of the own keys and of the prefix (-1: none; kJoint: the
 // sequences' items take the prefix's keys as well).
 // The 16- and 64-row kernels at head dim 64 are held to 128 registers, four waves a
-// SIMD: left alone the compiler takes 130 to 135, three (300 x 1 token over 512, 12
-// heads, 46.5 -> 42.7 us; 512 x 1 over 300, 57.2 -> 51.2; alike where a CU has up to
-// three workgroups).  None spills.
+// SIMD: left alone the compiler takes up to 133, three (300 x 1 token over 512, 12
+// heads, 46.5 us with three and 42.1 with four; 512 x 1 over 300, 57.3 and 53.4;
+// alike where a CU has up to three workgroups).  None spills.
 constexpr int kJoint = -2;
 template <int D, int V, int VP>
 __global__ __launch_bounds__(kThreads, D == 64 && V < 2 && VP < 2 ? 4 : 1) void cached_attn_kernel(CachedAttnArgs p) {

@@ -443,9 +443,11 @@ def cached_attention_hip(
 
     prefix: a cache of one sequence whose first prefix_length tokens stand
     before every sequence's own (at positions 0 .. prefix_length - 1, the own
-    ones behind them): a long one's keys and values are read once for the whole
-    batch.
-    starts still counts own tokens, and the window reaches back into the prefix.
+    ones behind them).  Where the sequences have few query rows each (generation,
+    drafts) a long one's keys and values are read once for the whole batch; a
+    short one's, or with sequences whose rows fill the kernel's tiles, once per
+    sequence.  starts still counts own tokens, and the window reaches back into
+    the prefix.
 
     Keys up to 2^119 and values up to 2^100 leave room for every sum; beyond,
     sums may overflow fp32.  No backward: q that requires grad is refused outside torch.no_grad()."""
