@@ -46,8 +46,9 @@
 // seen so far, 2^11 at p = 1, or to 2^8 times the row's own largest p_j vs_j if that
 // is less (a key of little weight may have a value far above the others): 11 bits
 // for weights above 2^-25 of it, and none above 2^-36 is lost.
-// Neither sum can pass fp32 while keys are below 2^119 (q.k_j with q at 2, D = 128)
-// and values below 2^100 (2^24 keys at up to 2^3).
+// Nothing passes fp32 while keys are below 2^119 (q.kc ks with q at 2, D = 128),
+// scale |q.k| below 2^127 (log2 units) and values below 2^100 (sums of 2^24 keys at
+// up to 2^3).
 #include <cmath>
 #include <utility>
 
@@ -208,7 +209,10 @@ struct Rows {
   int first, last;     // all keys that some row of the wave sees
   int inner_first, inner_last;  // the keys that every row sees
   f16x8 q[NT][C][2];
-  float rs[NT];             // scale log2(e) and q's power of two
+  // The power of two in scale log2(e) and q's: a row's scores (q.kc) ks times it are
+  // in log2 units, exactly, so that the largest one's probability is 1 however large
+  // it is.  The rest of scale log2(e), 0.5 .. 1, is in ks.
+  float rs[NT];
   float mt[NT], l[NT];      // running maximum of (q.kc) ks, sum
   // The value scale that each row's weights are relative to (0: none yet), and a
   // weight p vs that the row has seen, its largest when they were last looked at.
@@ -272,7 +276,7 @@ struct Rows {
       const int ex = min(126, max(-120, (top >> 7) - 127));
       const float down = __builtin_bit_cast(float, (127 - ex) << 23);
       // kept positive and finite: a score of -infinity times it stays what it is
-      rs[nt] = fminf(3e38f, fmaxf(1e-37f, p.scale_log2 * __builtin_bit_cast(float, (127 + ex) << 23)));
+      rs[nt] = __builtin_bit_cast(float, (127 + min(127, max(-126, ex + p.scale_exp))) << 23);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -288,7 +292,7 @@ struct Rows {
   }
 
   // Scores sc of block k0 .. k0 + 63 (before the keys' scales; ks, vs: those of
-  // key k0 + lane_key(lane)) into weights w, updating the rows' statistics.  Keys
+  // key k0 + lane_key(lane), ks with p.scale_part) into weights w, updating the rows' statistics.  Keys
   // of the block behind `end` are nobody's.
   __device__ __forceinline__ void weigh(f32x4 sc[NT][4], float ks, float vs, int k0, int end, int lane, f16x8 w[NT][2]) {
     const int g = lane >> 4;
@@ -474,7 +478,7 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
     const bool more = blk + NW < end;
     f32x4 sc[NT][4];
     f16x8 w[NT][2];
-    const float ks = ksl, vs = vsl;
+    const float ks = ksl * p.scale_part, vs = vsl;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       f16x8 kf[C][2];
@@ -642,7 +646,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
   __syncthreads();
   for (int blk = begin; blk < end; ++blk) {
     const int buf = (blk - begin) & 1;
-    const float ks = ks_next, vs = vs_next;
+    const float ks = ks_next * p.scale_part, vs = vs_next;
     if (blk + 1 < end) {
       store(buf ^ 1);
       load_scales(blk + 1);

@@ -788,7 +788,7 @@ int hlm_attn_cached_fwd(const void* q, const int64_t* q_strides, void* o, const 
   a.o = static_cast<hlm::bf16*>(o);
   a.own = cache(cache_k, cache_v, k_scale, v_scale, slots);
   a.prefix = cache(prefix_k, prefix_v, prefix_k_scale, prefix_v_scale, prefix_slots);
-  a.scale_log2 = scale * hlm::kLog2e;
+  a.scale_part = (float)std::frexp((double)scale * 1.4426950408889634, &a.scale_exp);
   a.div_G = hlm::fast_div_of((unsigned)a.G);
   a.div_T = hlm::fast_div_of((unsigned)T);
   a.part_o = static_cast<float*>(ws);

@@ -106,7 +106,8 @@ struct CachedAttnArgs {
   int B, H, Hkv, G;
   int P;       // prefix tokens
   int window;  // >= 1
-  float scale_log2;
+  float scale_part;  // scale log2(e) = scale_part 2^scale_exp, scale_part in 0.5 .. 1
+  int scale_exp;
   FastDiv div_G, div_T;
   int variant, prefix_variant;  // of the kernel, by its rows (-1: no prefix, -2: with the own keys)
   // Splits of the keys: own_splits workgroups share a sequence's keys (for one

@@ -840,3 +840,58 @@ def test_one_key_that_takes_it_all_with_a_small_value():
         cache, (kp, vp) = filled(g, 1, 512, 2, 64, k, v)
         out = hlm_attn.cached_attention_hip(q.cuda(), cache, 512 - T)
         check_by_weight(out, q, kp, vp, [512 - T], [T])
+
+
+# --- logits far from zero ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("T,Hkv", [(1, 2), (40, 2), (70, 1), (2000, 2)])
+def test_equal_logits_give_the_mean_however_large_they_are(T, Hkv):
+    """All keys alike in one dim: the probabilities are equal, the kernels' scores bit for bit, so that of a weight and of the
+    normaliser only the exponential of 0 and the fp16 weight are roundings.  Logits of 2^20 to 2^125, of either sign."""
+    g = torch.Generator().manual_seed(T)
+    S, D, H, P = 4096, 64, 4, 150
+    v = _rand(g, 1, S, Hkv, D) + 2
+    q, k = torch.zeros(1, T, H, D), torch.zeros(1, S, Hkv, D)
+    q[..., 0], k[..., 0] = 1.6875, 3.0
+    for sign in (1, -1):
+        cache, (_, (c, s)) = filled(g, 1, S, Hkv, D, (sign * k).bfloat16(), v)
+        pre, (_, (pc, ps)) = filled(g, 1, P, Hkv, D, (sign * k[:, :192]).bfloat16(), v[:, :192])
+        own, shared = c[0] * s[0, ..., None], pc[0, :, :P] * ps[0, :, :P, None]  # (Hkv, keys, D)
+        for power in (20, 26, 31, 60, 100, 122):
+            for prefix in (None, pre):
+                out = hlm_attn.cached_attention_hip(q.bfloat16().cuda(), cache, 333, scale=2.0**power, prefix=prefix, prefix_length=P if prefix else 0)
+                for t in {0, T // 2, T - 1}:
+                    for h in range(H):
+                        rows = own[h * Hkv // H, : 334 + t]
+                        rows = torch.cat((shared[h * Hkv // H], rows)) if prefix else rows
+                        n = rows.shape[0]
+                        want, size = rows.mean(0), rows.abs().mean(0)
+                        err = (out[0, t, h].double().cpu() - want).abs()
+                        assert (err <= 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-20 + n * 2.0**-23) * size).all(), (power, t, h)
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_a_far_larger_logit_takes_it_all(T):
+    """Logits that differ by 2^20 and more: each row's output is the value of its largest visible key."""
+    g = torch.Generator().manual_seed(T)
+    S, D, H, Hkv = 1024, 64, 4, 2
+    q, k = torch.zeros(1, T, H, D), torch.zeros(1, S, Hkv, D)
+    q[..., 0] = 1.25
+    k[0, :, :, 0] = torch.stack([torch.randperm(S, generator=g) for _ in range(Hkv)], 1) / 8 + 1.0  # apart by 2^-10 at least
+    k = k.bfloat16().float()
+    cache, ((kc, ks), (vc, vs)) = filled(g, 1, S, Hkv, D, k.bfloat16())
+    for scale in (2.0**34, 2.0**90):
+        for window in (None, 100):
+            out = hlm_attn.cached_attention_hip(q.bfloat16().cuda(), cache, S - T, window_size=window, scale=scale)
+            for t in {0, T // 2, T - 1}:
+                p = S - T + t
+                first = 0 if window is None else max(0, p - window + 1)
+                for h in range(H):
+                    g_ = h // (H // Hkv)
+                    logits = (kc[0, g_, first : p + 1, 0] * ks[0, g_, first : p + 1]) * 1.25
+                    best = (logits == logits.max()).nonzero()[:, 0] + first  # keys that bf16 made equal share it
+                    want = (vc[0, g_, best] * vs[0, g_, best, None]).mean(0)
+                    size = (vc[0, g_, best] * vs[0, g_, best, None]).abs().mean(0)
+                    err = (out[0, t, h].double().cpu() - want).abs()
+                    assert (err <= 2.0**-8 * want.abs() + (2.0**-10 + len(best) * 2.0**-23) * size + 1e-30).all(), (scale, t, h)
