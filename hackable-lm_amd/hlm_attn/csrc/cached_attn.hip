@@ -434,16 +434,16 @@ __device__ __forceinline__ void share(int first, int last, int split, int n_spli
   end = b0 + min(blocks, split * per + per);
 }
 
-// 16 NT rows, the keys shared by the four waves.
-template <int D, int NT, Segment SEG>
+// 16 rows, the keys shared by the four waves.
+template <int D, Segment SEG>
 __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
                                              bool partial, float* lds) {
-  constexpr int C = D / 64, DT = D / 16, ROWS = 16 * NT, LD = D + 4, NW = 4;
+  constexpr int C = D / 64, DT = D / 16, ROWS = 16, LD = D + 4, NW = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const int n_rows = SEG == kPrefix ? p.B * p.span.T * p.G : p.span.T * p.G;
   const Blocks<D, SEG> keys(p, unit);
-  Rows<D, NT> rows;
-  bf16x8 x_q[NT][C][2];
+  Rows<D, 1> rows;
+  bf16x8 x_q[1][C][2];
   rows.template begin<SEG>(p, unit, tile * ROWS, n_rows, lane, x_q);
   int begin, end;
   share(rows.first, rows.last, split, n_splits, begin, end);
@@ -478,8 +478,8 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
   rows.take_q(p, x_q);
   for (; blk < end; blk += NW) {
     const bool more = blk + NW < end;
-    f32x4 sc[NT][4];
-    f16x8 w[NT][2];
+    f32x4 sc[1][4];
+    f16x8 w[1][2];
     const float ks = ksl * p.scale_part, vs = vsl;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -488,26 +488,19 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int h = 0; h < 2; ++h) kf[c][h] = decode8(kr[t][c][2 * h], kr[t][c][2 * h + 1]);
+      sc[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) acc = mfma16(kf[c][h], rows.q[nt][c][h], acc);
-        sc[nt][t] = acc;
-      }
+        for (int h = 0; h < 2; ++h) sc[0][t] = mfma16(kf[c][h], rows.q[0][c][h], sc[0][t]);
     }
     if (more) load_k(blk + NW);
     rows.weigh(sc, ks, vs, blk * 64, keys.end(blk), lane, w);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const f16x8 v0 = decode8(vr[d][0], vr[d][1]), v1 = decode8(vr[d][2], vr[d][3]);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        rows.o[nt][d] = mfma16(v0, w[nt][0], rows.o[nt][d]);
-        rows.o[nt][d] = mfma16(v1, w[nt][1], rows.o[nt][d]);
-      }
+      rows.o[0][d] = mfma16(v0, w[0][0], rows.o[0][d]);
+      rows.o[0][d] = mfma16(v1, w[0][1], rows.o[0][d]);
     }
     if (more) load_v(blk + NW);
   }
@@ -516,29 +509,21 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
   float* ml = lds;                        // (NW, ROWS, 2)
   int* real = reinterpret_cast<int*>(lds + NW * ROWS * 2);  // (ROWS)
   float* sums = lds + NW * ROWS * 2 + ROWS;                 // (NW, ROWS, LD)
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float l = over_groups(rows.l[nt], Sum());
-    if (g == 0) {
-      float* at = ml + (wave * ROWS + 16 * nt + n) * 2;
-      at[0] = rows.top2(nt);
-      at[1] = l;
-      if (wave == 0) real[16 * nt + n] = rows.hi[nt] >= rows.lo[nt];
-    }
+  const float mine = rows.top2(0), l = over_groups(rows.l[0], Sum());
+  if (g == 0) {
+    float* at = ml + (wave * ROWS + n) * 2;
+    at[0] = mine;
+    at[1] = l;
+    if (wave == 0) real[n] = rows.hi[0] >= rows.lo[0];
   }
   __syncthreads();
+  float top = ml[n * 2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = 16 * nt + n;
-    float m = ml[r * 2];
+  for (int w = 1; w < NW; ++w) top = fmaxf(top, ml[(w * ROWS + n) * 2]);
+  const float f = mine == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mine - top) / kWeightTop;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) m = fmaxf(m, ml[(w * ROWS + r) * 2]);
-    const float mine = rows.top2(nt);
-    const float f = mine == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mine - m) / kWeightTop;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<f32x4*>(sums + (wave * ROWS + r) * LD + 16 * d + 4 * g) = rows.o[nt][d] * f * rows.ref[nt];
-  }
+  for (int d = 0; d < DT; ++d)
+    *reinterpret_cast<f32x4*>(sums + (wave * ROWS + n) * LD + 16 * d + 4 * g) = rows.o[0][d] * f * rows.ref[0];
   __syncthreads();
   constexpr int U = D / 4;
   for (int i = threadIdx.x; i < ROWS * U; i += 64 * NW) {
@@ -741,7 +726,7 @@ template <int D, int V, Segment SEG>
 __device__ __forceinline__ void attend(const CachedAttnArgs& p, int unit, int tile, int split, int n_splits, int slot,
                                        bool partial, float* lds) {
   if constexpr (V == 0)
-    attend_split<D, 1, SEG>(p, unit, tile, split, n_splits, slot, partial, lds);
+    attend_split<D, SEG>(p, unit, tile, split, n_splits, slot, partial, lds);
   else
     attend_tile<D, V, SEG>(p, unit, tile, split, n_splits, slot, partial, lds);
 }
