@@ -895,3 +895,47 @@ def test_a_far_larger_logit_takes_it_all(T):
                     size = (vc[0, g_, best] * vs[0, g_, best, None]).abs().mean(0)
                     err = (out[0, t, h].double().cpu() - want).abs()
                     assert (err <= 2.0**-8 * want.abs() + (2.0**-10 + len(best) * 2.0**-23) * size + 1e-30).all(), (scale, t, h)
+
+
+@pytest.mark.parametrize("prefix_tokens", [0, 70])
+def test_a_layer_step_is_captured_once_and_replayed(prefix_tokens):
+    """Projection, rotary tables at the tokens' places, forward_cached and the places' advance in one graph: each replay equals
+    the eager step of a twin cache, bit for bit, with that step between the replays."""
+    g = torch.Generator().manual_seed(24)
+    B, T, S = 3, 2, 192
+    cfg = hlm_attn.AttentionConfig(n_layer=2, n_head=4, n_kv_head=2, n_embd=64, attention_window=40, attention_full_every=2)
+    core, proj = hlm_attn.AttentionCore(cfg, 0), hlm_attn.QKVProjection(cfg, 0)
+    shared = filled(g, 1, prefix_tokens, 2, 64)[0] if prefix_tokens else None
+    with torch.no_grad():
+        proj.qkv_proj.weight.copy_(torch.randn(proj.qkv_proj.weight.shape, generator=g) * 0.1)
+        proj = proj.to("cuda", BF16)
+        proj.rope = hlm_attn.RotaryEmbedding(64).to("cuda")
+        places = torch.arange(T, device="cuda")
+        x, counts = torch.zeros(B, T, 64, dtype=BF16, device="cuda"), int32([T] * B)
+
+        def step(cache, starts):
+            rotary = proj.rope.at(starts[:, None] + places + prefix_tokens, BF16)
+            y = core.forward_cached(*proj(x, rotary), cache, starts, counts, shared, prefix_tokens)
+            starts += counts
+            return y
+
+        cache, twin = (hlm_attn.KVCache(B, S, 2, 64) for _ in range(2))
+        starts, twin_starts = int32([0] * B), int32([0] * B)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(twin, twin_starts)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(cache, starts)
+        twin_starts.zero_()
+        for n in ([2, 2, 2], [1, 2, 0], [2, 2, 2], [0, 1, 2], [2, 1, 1], [2, 2, 2]) * 3:
+            x.copy_(_rand(g, B, T, 64))
+            counts.copy_(int32(n))
+            graph.replay()
+            want = step(twin, twin_starts)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(starts, twin_starts)
+        for a, b in zip(hlm_attn.kv_cache_read_hip(cache, 0, S, starts), hlm_attn.kv_cache_read_hip(twin, 0, S, starts)):
+            assert torch.equal(a, b) and a.any()
