@@ -20,6 +20,8 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <strings.h>
@@ -100,6 +102,15 @@ bool plain(const at::Tensor& t) {
        c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Batched, c10::DispatchKey::Functionalize,
        c10::DispatchKey::ZeroTensor, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
   return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(kWrapped);
+}
+
+// Whether something active has to see the custom ops themselves, or may have to
+// (the caller looks closer then): a dispatch or function mode, a function
+// transform, jit tracing, forward-mode AD.
+bool watched() {
+  return c10::impl::TorchDispatchModeTLS::stack_len() > 0 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) ||
+         torch::jit::tracer::isTracing() || torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
 }
 
 // Whether a backward must go through its custom op: create_graph (the op then
@@ -458,6 +469,7 @@ PYBIND11_MODULE(_torch_fwd, m) {
   m.def("qk_norm_rope_train", &qk_norm_rope_train, "qk_norm_rope_train(q, k, cos, sin, eps) -> (q, k), or None");
   m.def("residual_rms_norm_train", &residual_rms_norm_train,
         "residual_rms_norm_train(residual, branch, eps) -> (out, normed), or None");
+  m.def("watched", &watched, "watched() -> whether a mode, a transform or tracing may have to see the custom ops");
   m.def("kv_cache_write", &kv_cache_write,
         "kv_cache_write(k, v, cache_k, cache_v, k_scale, v_scale, starts, start, counts) -> whether it was done");
   m.def("kv_cache_read", &kv_cache_read,

@@ -99,11 +99,16 @@ def _on_index(index: int):
     return torch.cuda.device(index)
 
 
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_function_modes = torch._C._len_torch_function_stack
+_transform = torch._C._functorch.peek_interpreter_stack
+_jit_tracing = torch._C._is_tracing
+
+
 def _ops_watched() -> bool:
     """Whether something active has to see the custom ops themselves: tracing,
     a dispatch mode, a function transform, forward-mode AD."""
-    return (torch.compiler.is_compiling() or bool(torch._C._len_torch_dispatch_stack())
-            or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._get_tracing_state() is not None
+    return (torch.compiler.is_compiling() or bool(_dispatch_modes()) or _transform() is not None or _jit_tracing()
             or forward_ad._current_level >= 0)
 
 
@@ -115,11 +120,14 @@ def direct_call_ok(*tensors: torch.Tensor) -> bool:
     needs a gradient (inference, e.g. the evaluation harness's no-grad
     forwards).  The dispatcher and autograd wrapper cost far more host time than
     the launch."""
-    if _ops_watched():
+    if torch.compiler.is_compiling():
         return False
-    if torch._C._len_torch_function_stack() and not all(
-            type(m) is DeviceContext for m in torch.overrides._get_current_function_mode_stack()):
-        return False
+    ext = _lib._torch_fwd
+    if not ext or ext.watched():  # one C++ call for the checks below (0.1 us against 0.4)
+        if _ops_watched():
+            return False
+        if _function_modes() and not all(type(m) is DeviceContext for m in torch.overrides._get_current_function_mode_stack()):
+            return False
     grad = torch.is_grad_enabled()
     for t in tensors:
         if type(t) is not torch.Tensor or (grad and t.requires_grad):
@@ -132,7 +140,7 @@ def eager_ext(*tensors: torch.Tensor):
     C++ autograd functions instead of the custom op, else None: plain tensors
     and parameters, and nothing active that has to see the op itself (tracing,
     a dispatch or function mode, a function transform, forward-mode AD)."""
-    if _ops_watched() or torch._C._len_torch_function_stack():
+    if _ops_watched() or _function_modes():
         return None
     for t in tensors:
         if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:

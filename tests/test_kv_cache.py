@@ -362,7 +362,10 @@ def _watched(f):
     torch.func.functionalize(lambda x: (f(x), x + 1)[1])(x)
 
 
-def test_direct_calls_stand_aside_where_the_op_must_be_seen():
+@pytest.mark.parametrize("extension", [True, False])
+def test_direct_calls_stand_aside_where_the_op_must_be_seen(monkeypatch, extension):
+    ext = _lib.load_torch_fwd()
+    monkeypatch.setattr(_lib, "_torch_fwd", ext if extension else False)
     x = torch.zeros(2, 3, 2, 64, dtype=BF16)
     taken = []
     with torch.no_grad():
@@ -370,7 +373,10 @@ def test_direct_calls_stand_aside_where_the_op_must_be_seen():
         assert taken == [False] * 7
         with torch.device("cpu"):  # a default device is a function mode that changes nothing for them
             assert ops.direct_call_ok(x)
-        assert ops.direct_call_ok(x)
+        assert ops.direct_call_ok(x) and not ext.watched()
+        taken.clear()
+        _watched(lambda x: taken.append(ext.watched()))
+        assert taken == [True] * 7
 
 
 def test_cache_calls_reach_their_ops_where_something_watches(monkeypatch):
