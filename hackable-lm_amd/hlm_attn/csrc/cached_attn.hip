@@ -20,12 +20,13 @@
 // rows' keys are joined by the combine kernel.
 //
 // Single tokens are bound by memory: 64 sequences of up to 2048 tokens, 12
-// heads of 64, 110.6 MB in 24.4 us (4.5 TB/s; a copy on this MI355X 4.8); 16384
-// keys of 16 heads of 128, 69 MB in 14.5 us and a join of 16 splits in 2 to 4.
-// Many rows are bound by the softmax's vector instructions, about 10 a score:
-// 2 x 500 tokens over 1500 and 2500, 12 heads of 64, 22.4 + 4.6 us.  A single
-// token over a window of 512 takes 5.3 us, most of it three trips to memory
-// (places, keys, rows of q with them) and the launch.
+// heads of 64, 110.6 MB in 24.6 us (4.5 TB/s; a copy on this MI355X 4.8); 16384
+// keys of 16 heads of 128, 69 MB in 14.8 us and a join of 16 splits in 3.9.  Many
+// rows are bound by the softmax's vector instructions, about 13 a score, of which
+// the exponential takes four slots: 2 x 500 tokens over 1500 and 2500, 12 heads of
+// 64, 23.3 + 4.6 us (each kernel alone).  A single token over a window of 512 takes
+// 5.3 us, most of it three trips to memory (places, keys, rows of q with them) and
+// the launch.
 //
 // Layouts (v_mfma_f32_16x16x32_f16, lane l, n = l % 16, g = l / 16):
 //   A (16 x 32): row n, k = 8 g + e;  B (32 x 16): k = 8 g + e, column n;
@@ -448,8 +449,8 @@ __device__ __forceinline__ void attend_split(const CachedAttnArgs& p, int unit, 
   int begin, end;
   share(rows.first, rows.last, split, n_splits, begin, end);
 
-  // Past the caches' retention, for own keys and values are read once (27.0 against
-  // 29.8 us for 64 sequences of up to 2048 tokens, 12 heads of 64).  A prefix's in
+  // Past the caches' retention, for own keys and values are read once (26.5 against
+  // 29.4 us for 64 sequences of up to 2048 tokens, 12 heads of 64).  A prefix's in
   // the joint pass are read by every sequence, and no slower so: 24 tokens over a
   // prefix of 60, 6 heads of 64, 6.7 us with either kind of load, 60 over 100 7.4 and 7.1.
   u32x4 kr[4][C], vr[DT];
@@ -703,7 +704,7 @@ __device__ __forceinline__ void attend_tile(const CachedAttnArgs& p, int unit, i
         p.part_ml[2 * at] = has ? rows.top2(nt) : -__builtin_inff();
         p.part_ml[2 * at + 1] = has ? l : 0.f;
       }
-      // past the caches' retention: 500 tokens over 1500 and 2500 27.6 -> 25.7 us
+      // past the caches' retention: 500 tokens over 1500 and 2500 28.4 -> 27.1 us
       // (the few rows of attend_split: 16384 keys of 16 heads 18.3 -> 18.6, so not there)
       if (has)
 #pragma unroll

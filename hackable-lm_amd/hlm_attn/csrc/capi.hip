@@ -615,7 +615,7 @@ int hlm_residual_rms_norm_bwd(const void* out, const void* grad_out, const void*
 
 namespace {
 
-constexpr int kMaxSlots = 1 << 24;  // a head's bytes, slots x 128, stay below 2^31
+constexpr int kMaxSlots = 1 << 24;  // a head's bytes, slots x 128, are at most 2^31; offsets into them are 64-bit
 
 // Strides of dims of one index are not looked at.
 int check_rows(const char* name, const void* p, const int64_t* s, int B, int T, int heads) {

@@ -11,9 +11,9 @@
 //
 // Memory-bound: 4 D bytes in and 2 (D + 4) out per token and head to write, the
 // reverse to read.  On an MI355X: 8 sequences of 1024 to 2048 tokens, 12 heads of
-// 64, written in 15.6 us (57.8 MB, 3.7 TB/s), read in 11.9 (70.4 MB with the
-// padding's zeros, 5.9 TB/s); 4 x 4096 tokens of 12 heads of 128 read in 24.0 us
-// (6.4 TB/s).  One token of 16 sequences: 4.0 and 3.4 us, a launch and one trip to
+// 64, written in 16.5 us (57.8 MB, 3.5 TB/s), read in 11.9 (70.4 MB with the
+// padding's zeros, 5.9 TB/s); 4 x 4096 tokens of 12 heads of 128 read in 24.9 us
+// (6.1 TB/s).  One token of 16 sequences: 4.1 and 3.4 us, a launch and one trip to
 // memory.
 #include "kv_cache.h"
 
@@ -117,9 +117,9 @@ __global__ __launch_bounds__(256) void cache_read_rows_kernel(CacheIoArgs p) {
 // threads take the keys, half the values; a thread holds 8 dims of 4 consecutive
 // tokens.  The image's 256-byte pieces are 272 bytes apart in LDS, so that the
 // lanes of a store fall on different banks (two to a bank at most).  bf16 rows
-// pass by the caches' retention, codes do not (8 sequences of up to 2048 tokens
-// written and read back: 31.9 us with neither, 28.9 with the loads past them,
-// 30.3 with the stores; with the codes' loads past them too, 30.3).
+// pass by the caches' retention (8 sequences of up to 2048 tokens written and read
+// back: 30.4 -> 28.3 us; 4 x 4096 of 12 heads of 128 read: 28.4 -> 25.4); codes do
+// not (1.4 us more for the former with their loads past them too).
 template <int D>
 struct Block {
   int64_t head;  // this head's first slot
