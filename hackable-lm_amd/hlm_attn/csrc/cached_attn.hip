@@ -47,9 +47,9 @@
 // seen so far, 2^11 at p = 1, or to 2^8 times the row's own largest p_j vs_j if that
 // is less (a key of little weight may have a value far above the others): 11 bits
 // for weights above 2^-25 of it, and none above 2^-36 is lost.
-// Nothing passes fp32 while keys are below 2^119 (q.kc ks with q at 2, D = 128),
-// scale |q.k| below 2^127 (log2 units) and values below 2^100 (sums of 2^24 keys at
-// up to 2^3).
+// Nothing passes fp32 while keys are at most 2^118 (q.kc ks with q at 4, D = 128),
+// scale |q| and scale |q.k| at most 2^126 (log2 units) and values at most 2^100
+// (sums of 2^24 keys at up to 2^3).
 #include <cmath>
 #include <utility>
 
@@ -275,9 +275,11 @@ struct Rows {
         }
       top = over_groups(top, Max());
       const int ex = min(126, max(-120, (top >> 7) - 127));
-      const float down = __builtin_bit_cast(float, (127 - ex) << 23);
-      // kept positive and finite: a score of -infinity times it stays what it is
-      rs[nt] = __builtin_bit_cast(float, (127 + min(127, max(-126, ex + p.scale_exp))) << 23);
+      // rs is kept positive and finite: a score of -infinity times it stays what it is.
+      // What is missing at 2^-126 makes q smaller (127 - ex + rest is 1 at least).
+      const int e = ex + p.scale_exp, rest = min(0, e + 126);
+      const float down = __builtin_bit_cast(float, (127 - ex + rest) << 23);
+      rs[nt] = __builtin_bit_cast(float, (127 + min(127, max(-126, e))) << 23);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll

@@ -449,9 +449,9 @@ def cached_attention_hip(
     sequence.  starts still counts own tokens, and the window reaches back into
     the prefix.
 
-    Keys up to 2^119, values up to 2^100 and scale |q.k| up to 2^126 leave room
-    for every sum; beyond, fp32 may overflow.  No backward: q that requires grad
-    is refused outside torch.no_grad()."""
+    Keys up to 2^118, values up to 2^100, scale |q| and scale |q.k| up to 2^126
+    leave room for every sum; beyond, fp32 may overflow.  No backward: q that
+    requires grad is refused outside torch.no_grad()."""
     ops = _ops or _load_ops()
     if window_size is not None:
         window_size = operator.index(window_size)  # half a token is no window

@@ -939,3 +939,47 @@ def test_a_layer_step_is_captured_once_and_replayed(prefix_tokens):
             assert torch.equal(out, want) and torch.equal(starts, twin_starts)
         for a, b in zip(hlm_attn.kv_cache_read_hip(cache, 0, S, starts), hlm_attn.kv_cache_read_hip(twin, 0, S, starts)):
             assert torch.equal(a, b) and a.any()
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("power,scale", [(-110, 2.0**-40), (-60, 2.0**-149), (-126, 2.0**-130), (-126, 2.0**20), (120, 2.0**-149), (127, 2.0**-140)])
+def test_queries_and_scales_at_the_ends_of_the_range(T, power, scale):
+    """Keys of 2^118 that all have the query's direction, half of them turned round: logits of +-scale |q.k|, from far below 2^-24
+    (the mean of all values) to a few units."""
+    g = torch.Generator().manual_seed(25)
+    S, D = 256, 128
+    q = torch.full((1, T, 2, D), 1.0) * 2.0**power
+    turned = torch.where(torch.arange(S) % 3 == 0, -1.0, 1.0)[None, :, None, None]
+    logit = scale * 2.0**power * D
+    size = 2.0**118 if logit * 2.0**118 < 8 else 4.0 / logit  # a power of two: exact codes
+    k = (turned * size).expand(1, S, 1, D)
+    cache, (kp, vp) = filled(g, 1, S, 1, D, k.bfloat16())
+    out = hlm_attn.cached_attention_hip(q.bfloat16().cuda(), cache, S - T, scale=scale)
+    values = vp[0][0, 0] * vp[1][0, 0, :, None]
+    for t in range(T):
+        p = torch.softmax((kp[0][0, 0, :, 0] * kp[1][0, 0] * scale * 2.0**power * D)[: S - T + t + 1], 0)
+        want, size_ = p @ values[: len(p)], p @ values[: len(p)].abs()
+        # logits up to 4: fp32 to (D + 4) 2^-24 of them, q in fp16 exact or, for the smallest, lost with logits below 2^-20
+        err = (out[0, t].double().cpu() - want).abs()
+        assert (err <= 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-13) * size_ + 1e-30).all(), t
+
+
+def test_a_prefix_of_no_tokens_many_query_heads_and_counts_past_the_end():
+    g = torch.Generator().manual_seed(26)
+    cache, (k, v) = filled(g, 3, 128, 1, 64)
+    q = _rand(g, 3, 2, 32, 64)
+    shared, _ = filled(g, 1, 64, 1, 64)
+    out = hlm_attn.cached_attention_hip(q.cuda(), cache, int32([5, 126, 60]), prefix=shared, prefix_length=0)
+    check_attention(out, q, k, v, [5, 126, 60], [2, 2, 2])
+    assert torch.equal(out, hlm_attn.cached_attention_hip(q.cuda(), cache, int32([5, 126, 60])))
+    # a place that the host knows, and more tokens than fit it: counts tell which are real, the cache's end which lie in it
+    for T in (12, 40):
+        q, counts = _rand(g, 3, T, 4, 64), [T, 3, 0]
+        out = hlm_attn.cached_attention_hip(q.cuda(), cache, 120, int32(counts))
+        check_attention(out, q, k, v, [120] * 3, counts)
+        x = _rand(g, 3, T, 1, 64)
+        hlm_attn.kv_cache_write_hip(cache, x.cuda(), x.cuda(), 120, int32(counts))
+        for c, s in (k, v):
+            oracle.write(c, s, x, [120] * 3, counts)
+        for got, (c, s) in zip(hlm_attn.kv_cache_read_hip(cache, 120, T, int32(counts)), (k, v)):
+            assert torch.equal(got.cpu(), oracle.read(c, s, T, [120] * 3, counts).float().bfloat16())
