@@ -295,8 +295,8 @@ struct Rows {
   }
 
   // Scores sc of block k0 .. k0 + 63 (before the keys' scales; ks, vs: those of
-  // key k0 + lane_key(lane), ks with p.scale_part) into weights w, updating the rows' statistics.  Keys
-  // of the block behind `end` are nobody's.
+  // key k0 + lane_key(lane), ks with p.scale_part) into weights w, updating the
+  // rows' statistics.  Keys of the block behind `end` are nobody's.
   __device__ __forceinline__ void weigh(f32x4 sc[NT][4], float ks, float vs, int k0, int end, int lane, f16x8 w[NT][2]) {
     const int g = lane >> 4;
     const bool whole = k0 >= inner_first && k0 + 63 <= min(inner_last, end);  // every row sees every key
